@@ -136,6 +136,53 @@ MS_API ms_status ms_q4_gemm(ms_ctx *ctx, const ms_q4_weight *w, float *C, const 
 MS_API ms_status ms_q4_gemm_noalloc(ms_ctx *ctx, const ms_q4_weight *w, float *C, const float *A,
                              int M, int accumulate, void *stream);
 
+/* ------------------------- 4-bit products with a scale per group of k */
+
+/* Element types of activations, results and logits of the calls that take a
+ * dtype. */
+enum { MS_F32 = 0, MS_BF16 = 1, MS_F16 = 2 };
+
+/* No counterpart in the reference, whose Q4 tensors have one scale each.
+ * A 4-bit matrix with one scale, and optionally one zero point, for every
+ * `group` values along k (32, 64 or 128):
+ *   w[k][n] = (q[k][n] - z[k / group][n]) * scale[k / group][n]
+ * w: [K][N / 2] bytes, low nibble = even column (the layout of
+ * ms_q4_weight_create); scales: [K / group][N] IEEE half (MS_F16) or bfloat16
+ * (MS_BF16); zeros: [K / group][N] bytes 0..15, or NULL (z = 8 everywhere).
+ * Host or device pointers, repacked once (waits for the device; the buffers
+ * may be freed afterwards).  K % group == 0, N % 2 == 0; a zero point above
+ * 15 is refused (MS_ERR_INVALID_ARG). */
+typedef struct ms_q4g_weight ms_q4g_weight;
+MS_API ms_status ms_q4g_weight_create(ms_ctx *ctx, const uint8_t *w, const void *scales,
+                               int scale_dtype, const uint8_t *zeros, int K, int N, int group,
+                               ms_q4g_weight **out);
+/* Waits for the device, then frees the weight. */
+MS_API ms_status ms_q4g_weight_destroy(ms_ctx *ctx, ms_q4g_weight *w);
+/* Device bytes the weight holds. */
+MS_API size_t ms_q4g_weight_bytes(const ms_q4g_weight *w);
+/* C[M,N] = A[M,K] . w (accumulate = 0) or C += A . w (accumulate = 1).
+ * A and C: device memory of one type (dtype), rows lda >= K and ldc >= N
+ * elements apart, aligned to their elements; they must not share memory.
+ * Activations are used exactly as given and sums are fp32, rounded once to
+ * dtype.  The call uses the context's workspace (rows of 16-bit limbs,
+ * M * K * 2 bytes per limb; 3 limbs for fp32, 2 for half, 1 for bfloat16):
+ * it grows on the first call of a size, which must not happen inside a
+ * stream capture (MS_ERR_STATE), and calls on different streams must not
+ * overlap in time, captured and replayed ones included. */
+MS_API ms_status ms_q4g_gemm(ms_ctx *ctx, const ms_q4g_weight *w, void *C, int64_t ldc,
+                      const void *A, int64_t lda, int dtype, int M, int accumulate,
+                      void *stream);
+/* Activation of the gate: x / (1 + e^-x), or
+ * x (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))) / 2. */
+enum { MS_ACT_SILU = 0, MS_ACT_GELU_TANH = 1 };
+/* H[M,N] = act(A . gate) * (A . up), the first half of a gated feed-forward
+ * block, in one kernel: neither product is written.  gate and up have the
+ * same K, N, group and scale type, and both or neither have zero points
+ * (MS_ERR_SHAPE otherwise).  The rest as ms_q4g_gemm. */
+MS_API ms_status ms_q4g_gated(ms_ctx *ctx, const ms_q4g_weight *gate, const ms_q4g_weight *up,
+                       int act, void *H, int64_t ldh, const void *A, int64_t lda, int dtype,
+                       int M, void *stream);
+
 /* ----------------------------------------------------------------- model */
 
 /* One decoder layer (E4BLayerRef, src/inference/gemma4_e4b.mojo:125-174;
@@ -384,6 +431,43 @@ MS_API void *ms_ctx_stream(ms_ctx *ctx);
 MS_API ms_status ms_sample(ms_ctx *ctx, const float *logits, int M, int V, const int *hist,
                            const int *hist_off, float temperature, float penalty,
                            const uint64_t *seeds, int *out_ids, void *stream);
+
+/* Rules on logits before sampling, for M rows of V ids (device memory; any
+ * part may be NULL / 0).  Row r, id j, c = occurrences of j in the row's
+ * history, in this order, fp32:
+ *   c > 0:                     v = (v > 0 ? v / repetition : v * repetition)
+ *                                  - (presence + frequency * c)
+ *   j in the row's bias list:  v = v + bias (an id listed twice: its last
+ *                              entry counts)
+ *   j's mask bit is 0:         v = -infinity, whatever v was
+ * Lists are CSR: row r's entries are off[r] .. off[r + 1] - 1, offsets
+ * clamped to 0 .. n; ids outside 0 .. V - 1 are skipped.  (ms_sample's own
+ * penalty divides once per occurrence, as the reference does; this one once
+ * per id.)  A row whose mask allows nothing is -infinity throughout. */
+typedef struct {
+  const int *hist;           /* [n_hist] ids                                 */
+  const int *hist_off;       /* [M + 1]                                      */
+  int n_hist;
+  const float *repetition;   /* [M], NULL = 1                                */
+  const float *presence;     /* [M], NULL = 0                                */
+  const float *frequency;    /* [M], NULL = 0                                */
+  const int *bias_id;        /* [n_bias] ids                                 */
+  const float *bias_val;     /* [n_bias]                                     */
+  const int *bias_off;       /* [M + 1]                                      */
+  int n_bias;
+  const uint32_t *mask;      /* [n_masks][mask_ld] words; bit j % 32 of word
+                                j / 32 allows id j                           */
+  int64_t mask_ld;           /* >= ceil(V / 32)                              */
+  int n_masks;
+  const int *mask_row;       /* [M] mask of each row, outside 0..n_masks - 1 =
+                                no mask; NULL: row r uses mask r             */
+} ms_logit_rules;
+/* out[r] = rules(logits[r]); rows ld and ldo elements apart, of one type
+ * (dtype).  out may be logits itself (then ld == ldo), else the two must not
+ * overlap.  M <= 65535.  Asynchronous; no workspace. */
+MS_API ms_status ms_logit_rules_apply(ms_ctx *ctx, const void *logits, int64_t ld, void *out,
+                               int64_t ldo, int dtype, int M, int V,
+                               const ms_logit_rules *rules, void *stream);
 
 /* Sampling of the token loop (ms_decode_step, ms_generate and ms_prefill's
  * first ids; the reference's loop calls temperature_sampling with T = 0.7,

@@ -59,6 +59,15 @@ class LoadOpts(ctypes.Structure):
                 ("staging_bytes", ctypes.c_size_t)]
 
 
+class LogitRulesDesc(ctypes.Structure):
+    """ms_logit_rules."""
+    _fields_ = [("hist", _vp), ("hist_off", _vp), ("n_hist", ctypes.c_int),
+                ("repetition", _vp), ("presence", _vp), ("frequency", _vp),
+                ("bias_id", _vp), ("bias_val", _vp), ("bias_off", _vp), ("n_bias", ctypes.c_int),
+                ("mask", _vp), ("mask_ld", ctypes.c_int64), ("n_masks", ctypes.c_int),
+                ("mask_row", _vp)]
+
+
 # name -> (restype, argtypes); every symbol include/mojostream_cuda.h declares
 SIGNATURES = {
     "ms_abi_version": (ctypes.c_int, []),
@@ -75,6 +84,14 @@ SIGNATURES = {
     "ms_q4_weight_destroy": (ctypes.c_int, [_vp, _vp]),
     "ms_q4_gemm": (ctypes.c_int, [_vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int, _vp]),
     "ms_q4_gemm_noalloc": (ctypes.c_int, [_vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int, _vp]),
+    "ms_q4g_weight_create": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int, _vp, ctypes.c_int,
+                                            ctypes.c_int, ctypes.c_int, ctypes.POINTER(_vp)]),
+    "ms_q4g_weight_destroy": (ctypes.c_int, [_vp, _vp]),
+    "ms_q4g_weight_bytes": (ctypes.c_size_t, [_vp]),
+    "ms_q4g_gemm": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int64, _vp, ctypes.c_int64,
+                                   ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp]),
+    "ms_q4g_gated": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int, _vp, ctypes.c_int64, _vp,
+                                    ctypes.c_int64, ctypes.c_int, ctypes.c_int, _vp]),
     "ms_model_create": (ctypes.c_int, [_vp, ctypes.POINTER(ModelDesc), ctypes.POINTER(_vp)]),
     "ms_model_destroy": (ctypes.c_int, [_vp, _vp]),
     "ms_model_weight_bytes": (ctypes.c_size_t, [_vp]),
@@ -114,6 +131,9 @@ SIGNATURES = {
     "ms_prefill": (ctypes.c_int, [_vp, _vp, _vp, _ip, _ip, _ip, ctypes.c_int, _ip]),
     "ms_sample": (ctypes.c_int, [_vp, _vp, ctypes.c_int, ctypes.c_int, _vp, _vp, ctypes.c_float,
                                  ctypes.c_float, _vp, _vp, _vp]),
+    "ms_logit_rules_apply": (ctypes.c_int, [_vp, _vp, ctypes.c_int64, _vp, ctypes.c_int64,
+                                            ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                            ctypes.POINTER(LogitRulesDesc), _vp]),
     "ms_set_sampling": (ctypes.c_int, [_vp, _vp, ctypes.c_float, ctypes.c_float,
                                        ctypes.c_uint64]),
     "ms_tp_unique_id_bytes": (ctypes.c_size_t, []),

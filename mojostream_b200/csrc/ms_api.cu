@@ -33,6 +33,8 @@
 #include "ms_kernels.h"
 #include "ms_pages.h"
 #include "ms_plan.h"
+#include "ms_q4g.h"
+#include "ms_rules.h"
 
 using namespace ms;
 
@@ -63,6 +65,11 @@ struct ms_ctx {
   // ms_sample: chunk partials and per-row arrival tickets (grown on demand)
   float2* samp_part = nullptr;
   size_t samp_part_n = 0;
+  // operators beside the token loop: one workspace, and the smaller ones that
+  // it replaced (captured graphs may hold them)
+  void* ws = nullptr;
+  size_t ws_bytes = 0;
+  std::vector<void*> ws_old;
   double load_secs = 0.0;  // last ms_model_load: reads + host-to-device copies
   uint64_t load_bytes = 0;
   int* samp_cnt = nullptr;
@@ -362,7 +369,8 @@ extern "C" ms_status ms_init(int device, ms_ctx** out) {
   cudaEventCreate(&c->ev[1]);
   if (prepare_gemv_stream() != cudaSuccess || prepare_attention() != cudaSuccess ||
       prepare_gemm_tc() != cudaSuccess || prepare_gemm_sk() != cudaSuccess ||
-      prepare_lm_tc() != cudaSuccess ||
+      prepare_lm_tc() != cudaSuccess || prepare_q4g() != cudaSuccess ||
+      prepare_rules() != cudaSuccess ||
       prepare_attention_prefill() != cudaSuccess) {
     ms_destroy(c);
     return MS_ERR_CUDA;
@@ -389,6 +397,8 @@ extern "C" ms_status ms_destroy(ms_ctx* c) {
   cudaFree(c->rowf);
   cudaFree(c->samp_part);
   cudaFree(c->samp_cnt);
+  cudaFree(c->ws);
+  for (void* p : c->ws_old) cudaFree(p);
   if (c->comm) nccl_api().comm_destroy(c->comm);
   if (c->ev[0]) cudaEventDestroy(c->ev[0]);
   if (c->ev[1]) cudaEventDestroy(c->ev[1]);
@@ -399,11 +409,33 @@ extern "C" ms_status ms_destroy(ms_ctx* c) {
 
 extern "C" const char* ms_last_error(const ms_ctx* c) { return c ? c->err.c_str() : "null context"; }
 
-// ------------------------------------------------- internal (ms_loader.cu) --
+// -------------------------------------- internal (ms_loader.cu, ms_ops.cu) --
 
 ms_status ms_fail_(ms_ctx* c, ms_status s, const char* msg) { return fail(c, s, "%s", msg); }
 cudaStream_t ms_stream_(ms_ctx* c) { return c->stream; }
 int ms_device_(const ms_ctx* c) { return c->device; }
+int ms_sm_count_(const ms_ctx* c) { return c->sm_count; }
+int* ms_err_word_(ms_ctx* c) { return c->d_err; }
+
+ms_status ms_workspace_(ms_ctx* c, cudaStream_t s, size_t bytes, void** out) {
+  if (bytes > c->ws_bytes) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    MS_CUDA(c, cudaStreamIsCapturing(s, &cap));
+    if (cap != cudaStreamCaptureStatusNone)
+      return fail(c, MS_ERR_STATE,
+                  "the workspace (%zu bytes) would have to grow to %zu inside a stream capture: "
+                  "make one call of this size before it", c->ws_bytes, bytes);
+    const size_t want = std::max(std::max(bytes, 2 * c->ws_bytes), (size_t)1 << 20);
+    void* p = nullptr;
+    MS_TRY(dev_alloc(c, &p, want));
+    if (c->ws) c->ws_old.push_back(c->ws);
+    c->ws = p;
+    c->ws_bytes = want;
+  }
+  *out = c->ws;
+  return MS_OK;
+}
+
 void ms_set_load_stats_(ms_ctx* c, double seconds, uint64_t bytes) {
   c->load_secs = seconds;
   c->load_bytes = bytes;

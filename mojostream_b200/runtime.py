@@ -53,6 +53,45 @@ def _stream():
     return ctypes.c_void_p(s if s else _CUDA_STREAM_LEGACY)
 
 
+def _stream_on(device):
+    """torch's current stream of `device` (see _stream), whichever device is
+    current."""
+    import torch
+    s = torch.cuda.current_stream(device).cuda_stream
+    return s if s else _CUDA_STREAM_LEGACY
+
+
+_DTYPES = None
+
+
+def _dtype_code(t, what):
+    """MS_F32 / MS_BF16 / MS_F16 of a tensor."""
+    global _DTYPES
+    if _DTYPES is None:
+        import torch
+        _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what}: float32, bfloat16 or float16 needed, got {t.dtype}")
+    return code
+
+
+def _check_2d(t, what, device, cols=None, rows=None):
+    """A row-strided matrix of `device` handed to the C-ABI: rows any number
+    of elements apart, the elements of a row adjacent."""
+    if not getattr(t, "is_cuda", False) or t.device.index != device:
+        raise ValueError(f"{what}: a tensor on CUDA device {device} is needed")
+    shape = t.shape
+    if len(shape) != 2 or (cols is not None and shape[1] != cols) or (rows is not None and shape[0] != rows):
+        raise ValueError(f"{what}: shape {tuple(shape)}, need ({'M' if rows is None else rows}, "
+                         f"{'V' if cols is None else cols})")
+    st = t.stride()
+    ld = st[0] if shape[0] > 1 else max(st[0], shape[1])
+    if (st[1] != 1 and shape[1] > 1) or ld < shape[1]:
+        raise ValueError(f"{what}: rows of adjacent elements needed, got strides {st}")
+    return ld
+
+
 def tp_unique_id():
     """A fresh tensor-parallel group id (ms_tp_unique_id), made by rank 0."""
     n = lib().ms_tp_unique_id_bytes()
@@ -108,6 +147,24 @@ class Context:
                                    _stream()))
         return out
 
+    def logit_rules(self, logits, rules, out=None):
+        """ms_logit_rules_apply: penalties, biases and masks (a LogitRules) on
+        a CUDA tensor [M][V] of float32, bfloat16 or float16 logits, rows of
+        any stride.  out: None (in place), or a tensor of the same shape and
+        type.  Returns the tensor written."""
+        if out is None:
+            out = logits
+        M, V = logits.shape if logits.dim() == 2 else (0, 0)
+        ld = _check_2d(logits, "logits", self.device)
+        ldo = _check_2d(out, "out", self.device, V, M)
+        code = _dtype_code(logits, "logits")
+        if out.dtype != logits.dtype:
+            raise ValueError(f"out: {logits.dtype} needed, got {out.dtype}")
+        rules.check(M, V, self.device)
+        self.check(lib().ms_logit_rules_apply(self.h, logits.data_ptr(), ld, out.data_ptr(), ldo,
+                                              code, M, V, rules.ref, _stream_on(self.device)))
+        return out
+
     def tp_init(self, world, rank, unique_id):
         """Join a tensor-parallel group of `world` ranks (ms_tp_init); call
         before creating models.  unique_id: the bytes of tp_unique_id() made
@@ -159,6 +216,158 @@ class Q4Weight:
             self.close()
         except Exception:
             pass
+
+
+class Q4GroupWeight:
+    """ms_q4g_weight: a 4-bit matrix with a scale, and optionally a zero
+    point, per group of 32, 64 or 128 values along k."""
+
+    def __init__(self, ctx, w_rx, scales, K, N, group, zeros=None):
+        """w_rx: uint8 [K][N / 2] (low nibble = even column); scales: float16
+        or bfloat16 [K / group][N]; zeros: uint8 [K / group][N] of 0..15, or
+        None (8 everywhere).  NumPy or torch, host or device."""
+        if group not in (32, 64, 128) or K <= 0 or N <= 0 or K % group or N % 2:
+            raise ValueError(f"K {K}, N {N}, group {group}: K % group == 0, N % 2 == 0 and a "
+                             "group of 32, 64 or 128 needed")
+        self.ctx, self.K, self.N, self.group = ctx, K, N, group
+        code = {"float16": 2, "bfloat16": 1}.get(str(scales.dtype).replace("torch.", ""))
+        if code is None:
+            raise ValueError(f"scales: float16 or bfloat16 needed, got {scales.dtype}")
+        for t, what, shape in ((w_rx, "w_rx", (K, N // 2)), (scales, "scales", (K // group, N)),
+                               (zeros, "zeros", (K // group, N))):
+            if t is None:
+                continue
+            if tuple(t.shape) != shape:
+                raise ValueError(f"{what}: shape {tuple(t.shape)}, need {shape}")
+            if what != "scales" and str(t.dtype).replace("torch.", "") != "uint8":
+                raise ValueError(f"{what}: uint8 needed, got {t.dtype}")
+        keep = [np.ascontiguousarray(t) if isinstance(t, np.ndarray) else None if t is None
+                else t.contiguous() for t in (w_rx, scales, zeros)]
+        h = ctypes.c_void_p()
+        ctx.check(lib().ms_q4g_weight_create(ctx.h, _ptr(keep[0]), _ptr(keep[1]), code,
+                                             None if zeros is None else _ptr(keep[2]), K, N, group,
+                                             ctypes.byref(h)))
+        self.h = h
+
+    @property
+    def nbytes(self):
+        """Device bytes of the weight."""
+        return lib().ms_q4g_weight_bytes(self.h)
+
+    def gemm(self, A, C, accumulate=False):
+        """C = A . w, or C += A . w (ms_q4g_gemm): A [M][K] and C [M][N] of one
+        type (float32, bfloat16, float16), rows of any stride."""
+        ctx = self.ctx
+        lda = _check_2d(A, "A", ctx.device, self.K)
+        ldc = _check_2d(C, "C", ctx.device, self.N, A.shape[0])
+        code = _dtype_code(A, "A")
+        if C.dtype != A.dtype:
+            raise ValueError(f"C: {A.dtype} needed, got {C.dtype}")
+        ctx.check(lib().ms_q4g_gemm(ctx.h, self.h, C.data_ptr(), ldc, A.data_ptr(), lda, code,
+                                    A.shape[0], 1 if accumulate else 0, _stream_on(ctx.device)))
+        return C
+
+    def gated(self, up, A, H, act="silu"):
+        """H = act(A . self) * (A . up) in one kernel (ms_q4g_gated): the first
+        half of a gated feed-forward block; act "silu" or "gelu_tanh"."""
+        ctx = self.ctx
+        lda = _check_2d(A, "A", ctx.device, self.K)
+        ldh = _check_2d(H, "H", ctx.device, self.N, A.shape[0])
+        code = _dtype_code(A, "A")
+        if H.dtype != A.dtype:
+            raise ValueError(f"H: {A.dtype} needed, got {H.dtype}")
+        kind = {"silu": 0, "gelu_tanh": 1}.get(act)
+        if kind is None:
+            raise ValueError(f"act {act!r}: silu or gelu_tanh")
+        ctx.check(lib().ms_q4g_gated(ctx.h, self.h, up.h, kind, H.data_ptr(), ldh, A.data_ptr(),
+                                     lda, code, A.shape[0], _stream_on(ctx.device)))
+        return H
+
+    def close(self):
+        if getattr(self, "h", None):
+            lib().ms_q4g_weight_destroy(self.ctx.h, self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class LogitRules:
+    """ms_logit_rules: what Context.logit_rules applies to rows of logits.
+    Device tensors, kept (not copied): a caller may change their values
+    between calls."""
+
+    _INT = ("hist", "hist_off", "bias_id", "bias_off", "mask", "mask_row")
+
+    def __init__(self, hist=None, hist_off=None, repetition=None, presence=None, frequency=None,
+                 bias_id=None, bias_val=None, bias_off=None, mask=None, mask_row=None):
+        """hist [n] int32 ids of all rows with hist_off [M + 1] int32;
+        repetition, presence, frequency [M] float32; bias_id [n] int32 and
+        bias_val [n] float32 with bias_off [M + 1] int32; mask [n_masks][words]
+        int32 (bit j % 32 of word j / 32 allows id j) and mask_row [M] int32
+        (-1: no mask; None: row r uses mask r)."""
+        given = dict(hist=hist, hist_off=hist_off, repetition=repetition, presence=presence,
+                     frequency=frequency, bias_id=bias_id, bias_val=bias_val, bias_off=bias_off,
+                     mask=mask, mask_row=mask_row)
+        self.tensors = {}
+        d = _lib.LogitRulesDesc()
+        self.device = None
+        for name, t in given.items():
+            if t is None:
+                continue
+            want = "torch.int32" if name in self._INT else "torch.float32"
+            if not getattr(t, "is_cuda", False) or str(t.dtype) != want:
+                raise ValueError(f"{name}: a CUDA tensor of {want} needed")
+            if not t.is_contiguous() or t.dim() != (2 if name == "mask" else 1):
+                raise ValueError(f"{name}: a contiguous tensor of {2 if name == 'mask' else 1} "
+                                 "dimension(s) needed")
+            if self.device not in (None, t.device.index):
+                raise ValueError(f"{name}: on device {t.device.index}, others on {self.device}")
+            self.device = t.device.index
+            self.tensors[name] = t
+            if t.numel():
+                setattr(d, name, t.data_ptr())
+        for group in (("hist", "hist_off"), ("bias_id", "bias_val", "bias_off")):
+            have = [n in self.tensors for n in group]
+            if any(have) and not all(have):
+                raise ValueError(f"{', '.join(group)} go together")
+        if "bias_id" in self.tensors and bias_id.numel() != bias_val.numel():
+            raise ValueError(f"bias_val: {bias_val.numel()} values for {bias_id.numel()} ids")
+        if "hist" not in self.tensors and any(
+                n in self.tensors for n in ("repetition", "presence", "frequency")):
+            raise ValueError("penalties need hist and hist_off")
+        if "mask_row" in self.tensors and "mask" not in self.tensors:
+            raise ValueError("mask_row needs mask")
+        d.n_hist = hist.numel() if "hist" in self.tensors else 0
+        d.n_bias = bias_id.numel() if "bias_id" in self.tensors else 0
+        # an empty list and its offsets are left out
+        if not d.n_hist:
+            d.hist = d.hist_off = d.repetition = d.presence = d.frequency = None
+        if not d.n_bias:
+            d.bias_id = d.bias_val = d.bias_off = None
+        if "mask" in self.tensors:
+            d.n_masks, d.mask_ld = mask.shape
+        self.desc = d
+        self.ref = ctypes.byref(d)
+
+    def check(self, M, V, device):
+        """The lengths that M rows of V ids need."""
+        if self.device not in (None, device):
+            raise ValueError(f"rules on device {self.device}, logits on {device}")
+        for name, t in self.tensors.items():
+            if name == "mask":
+                if t.shape[1] * 32 < V:
+                    raise ValueError(f"mask: {t.shape[1]} words for {V} ids")
+                if "mask_row" not in self.tensors and t.shape[0] < M:
+                    raise ValueError(f"mask: {t.shape[0]} masks for {M} rows without mask_row")
+            elif name in ("hist_off", "bias_off"):
+                if t.numel() != M + 1:
+                    raise ValueError(f"{name}: {t.numel()} offsets for {M} rows")
+            elif name not in ("hist", "bias_id", "bias_val") and t.numel() != M:
+                raise ValueError(f"{name}: {t.numel()} values for {M} rows")
 
 
 class Model:
