@@ -112,44 +112,28 @@ ms_status run_q4g(ms_ctx* c, const ms_q4g_weight* w, const ms_q4g_weight* w2, in
   Q4gParams p{};
   p.w = w->v;
   p.w2 = w2 ? w2->v.w : nullptr;
-  p.limbs = qg_limbs(dtype);
-  p.M = M;
+  p.a.a = a;
+  p.a.lda = lda;
+  p.a.type = dtype;
+  p.a.M = M;
+  p.a.K = w->v.K;
+  p.a.nkb = w->v.nkb;
+  p.a.group = w->v.group;
+  p.a.vec = !((uintptr_t)a & 15) && (lda * type_size(dtype)) % 16 == 0;
   p.out = out;
   p.ldo = ldo;
-  p.type = dtype;
   p.accumulate = accumulate;
   p.act = act;
   p.err = ms_err_word_(c);
-  const int NB = M <= 8 ? 1 : 2;
-  p.mb = M <= NB * 8 ? M : NB * 8;
-  if ((M + p.mb - 1) / p.mb > 65535) OPS_FAIL(c, MS_ERR_SHAPE, "q4g: M=%d", M);
-  const int R = p.mb * p.limbs;
-  int T = NB == 2 ? 2 : R <= 3 ? 1 : R <= 8 ? 2 : 4;
-  if (w2 && T < 2) T = 2;
-  const int kpad = w->v.nkb * kQgBlockK;
-  // one bfloat16 row is its own limb plane
-  if (M == 1 && dtype == MS_BF16 && w->v.K == kpad && !((uintptr_t)a & 15)) {
-    p.planes = (const uint8_t*)a;
-  } else {
+  if ((M + kQgMaxRows - 1) / kQgMaxRows > 65535) OPS_FAIL(c, MS_ERR_SHAPE, "q4g: M=%d", M);
+  if (!q4g_stream_converts(p, ms_sm_count_(c))) {
     void* ws = nullptr;
-    const size_t bytes = (size_t)M * p.limbs * kpad * 2;
-    const ms_status st = ms_workspace_(c, s, bytes, &ws);
+    const ms_status st = ms_workspace_(c, s, q4g_records_bytes(p.a), &ws);
     if (st != MS_OK) return st;
-    Q4gPlanes q{};
-    q.a = a;
-    q.lda = lda;
-    q.type = dtype;
-    q.M = M;
-    q.K = w->v.K;
-    q.kpad = kpad;
-    q.mb = p.mb;
-    q.limbs = p.limbs;
-    q.vec = !((uintptr_t)a & 15) && (lda * type_size(dtype)) % 16 == 0;
-    q.planes = (uint8_t*)ws;
-    p.planes = q.planes;
-    OPS_CUDA(c, launch_q4g_planes(q, s));
+    p.a.records = (uint8_t*)ws;
+    OPS_CUDA(c, launch_q4g_rows(p.a, s));
   }
-  OPS_CUDA(c, launch_q4g_stream(p, T, NB, ms_sm_count_(c), s));
+  OPS_CUDA(c, launch_q4g_stream(p, ms_sm_count_(c), s));
   return MS_OK;
 }
 

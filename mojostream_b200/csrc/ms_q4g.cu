@@ -1,13 +1,15 @@
 // ms_q4g.cu -- products with group-scaled 4-bit weights (layout: ms_q4g.h):
 //   C[m][n] (+)= sum_k A[m][k] (q[k][n] - z) s,   H = act(A Wg) * (A Wu).
 //
-// Mathematics.  q - z is an integer of at most 5 bits: exact in bfloat16
-// ((0x4300 | q) is the bfloat16 128 + q; subtracting 128 + z leaves q - z).
-// An activation is cut into bfloat16 limbs that add up to it exactly (fp32:
-// 8 + 8 + 8 bits, fp16: 8 + 3, bfloat16: itself), so every product of the
-// mma.m16n8k16 is exact and its fp32 accumulator holds the sum of one group;
-// the group's scale is applied in fp32 when the group ends.  All limbs of a
-// row add into the same accumulator.
+// Decode rows run on integer tensor cores: activations as signed 8-bit digits
+// relative to their group's largest value (ms_q4g.h), so that
+//   sum_k (q - z) a = sum_l f_l (sum_k q d_l - z sum_k d_l)
+// with exact integer sums per group (|sum| < 2^23, exact in fp32 too); group
+// scales, digit factors and groups are applied and added in fp32.  Unpacking
+// costs two ANDs for eight weights; the same product with weights expanded to
+// bfloat16 took seven shifts and logic operations and four subtractions for
+// them, and that, not memory, was its bound (K 2560, N 262144, one row:
+// 109 us against 53 us of bytes).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -20,6 +22,39 @@ namespace {
 
 __device__ __forceinline__ float u16_scale(uint32_t u, int bf) {
   return bf ? __uint_as_float(u << 16) : __half2float(__ushort_as_half((unsigned short)u));
+}
+
+// Shared-memory loads by 32-bit address.
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t a) {
+  uint32_t v;
+  asm volatile("{\n .reg .u16 h;\n ld.shared.u16 h, [%1];\n cvt.u32.u16 %0, h;\n}" : "=r"(v) : "r"(a));
+  return v;
+}
+
+// D = A (16 x 32, unsigned bytes) * B (32 x 8, signed bytes) + C, exact in s32.
+__device__ __forceinline__ void mma_u8s8_16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                               uint32_t a3, uint32_t b0, uint32_t b1,
+                                               const int (&c)[4]) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]),
+        "r"(c[3]));
 }
 
 // ------------------------------------------------------------- repack --
@@ -75,97 +110,149 @@ __global__ void q4g_repack_kernel(uint8_t* __restrict__ out, const Q4gView v,
   }
 }
 
-// -------------------------------------------------------------- planes --
-// v = hi + mid + lo exactly: each limb is the leading 8 bits of what is left
-// (truncated, so nothing can round up to infinity).  An infinity or a NaN
-// stays in the first limb alone.
-__device__ __forceinline__ void limbs3(float v, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
-  const uint32_t u = __float_as_uint(v);
-  hi = u & 0xffff0000u;
-  float r = v - __uint_as_float(hi);
-  if ((u & 0x7f800000u) == 0x7f800000u) {
-    if (u & 0x007fffffu) hi |= 0x00400000u;  // a NaN whose payload sits in the low bits
-    r = 0.f;
+// ----------------------------------------------------- rows to records --
+// Eight consecutive values of a row (zeros past K, a multiple of 32).
+__device__ __forceinline__ void load8(const Q4gRows& a, int m, int k, float (&v)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = 0.f;
+  if (k >= a.K) return;
+  if (a.type == kQgF32) {
+    const float* x = reinterpret_cast<const float*>(a.a) + (size_t)m * a.lda + k;
+    if (a.vec) {
+      const float4 y = __ldcg(reinterpret_cast<const float4*>(x));
+      const float4 z = __ldcg(reinterpret_cast<const float4*>(x) + 1);
+      v[0] = y.x; v[1] = y.y; v[2] = y.z; v[3] = y.w;
+      v[4] = z.x; v[5] = z.y; v[6] = z.z; v[7] = z.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = __ldcg(x + j);
+    }
+  } else {
+    const unsigned short* x = reinterpret_cast<const unsigned short*>(a.a) + (size_t)m * a.lda + k;
+    uint32_t u[8];
+    if (a.vec) {
+      const uint4 y = __ldcg(reinterpret_cast<const uint4*>(x));
+      const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[j] = (w[j / 2] >> (16 * (j & 1))) & 0xffffu;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[j] = __ldcg(x + j);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      v[j] = a.type == kQgBf16 ? __uint_as_float(u[j] << 16)
+                               : __half2float(__ushort_as_half((unsigned short)u[j]));
   }
-  mid = __float_as_uint(r) & 0xffff0000u;
-  lo = __float_as_uint(r - __uint_as_float(mid));  // at most 8 bits: exact
 }
 
-// Thread: 8 k of one row.  Grid x over k / 32 pieces of 4 threads, y over rows
-// of the padded row blocks.
-__global__ void __launch_bounds__(256) q4g_planes_kernel(const Q4gPlanes p) {
-  pdl_wait();     // the activations are an earlier kernel's output, and the
-  pdl_trigger();  // planes may still be read by the product before this one
-  const int k8 = blockIdx.x * blockDim.x + threadIdx.x;
-  if (k8 * 8 >= p.kpad) return;
-  for (int m = blockIdx.y; m < p.M; m += gridDim.y) {
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// Byte l of four digit words, k order {0, 2, 1, 3}, for l = 0..3.
+__device__ __forceinline__ void transpose4(const uint32_t* d, uint32_t (&w)[4]) {
+  const uint32_t lo0 = __byte_perm(d[0], d[2], 0x5140), lo1 = __byte_perm(d[1], d[3], 0x5140);
+  const uint32_t hi0 = __byte_perm(d[0], d[2], 0x7362), hi1 = __byte_perm(d[1], d[3], 0x7362);
+  w[0] = __byte_perm(lo0, lo1, 0x5410);
+  w[1] = __byte_perm(lo0, lo1, 0x7632);
+  w[2] = __byte_perm(hi0, hi1, 0x5410);
+  w[3] = __byte_perm(hi0, hi1, 0x7632);
+}
+
+// Sixteen lanes: 128 k of a row, 8 consecutive ones (v) per lane hl, into
+// columns c0 .. c0 + 3 of a record with `cols` columns.  Whole warp (two
+// rows or blocks at a time); nothing is written where live is false.
+//   A group with a NaN gets the factor NaN; one with infinities holds +-1 at
+// them, 0 elsewhere and the factor infinity, so that infinity * w comes out
+// as it should (NaN for w = 0).
+__device__ __forceinline__ void convert8(const float (&v)[8], int group, int c0, int cols, int hl,
+                                         bool live, uint8_t* rec) {
+  const int glanes = group / 8, ng = kQgBlockK / group;
+  const int c8 = (cols + 7) / 8 * 8;
+  uint32_t mx = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) mx = max(mx, __float_as_uint(v[j]) & 0x7fffffffu);
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, mx, o);
+    if (o < glanes) mx = max(mx, other);
+  }
+  // exponent of the largest value; groups below 2^-90 share its scale
+  constexpr int top = 29;
+  const int e = max((int)(mx >> 23) - 127, -90);
+  const bool finite = mx < 0x7f800000u;
+  const float up = finite ? pow2(top - e) : 0.f;
+  uint32_t d[8];  // the digits of q: q + 0x80808080 with every byte's top bit flipped
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    int q = __float2int_rn(v[j] * up);
+    if (!finite) q = isinf(v[j]) ? (v[j] > 0.f ? 1 : -1) : 0;
+    d[j] = ((uint32_t)q + 0x80808080u) ^ 0x80808080u;
+  }
+  uint32_t w0[4], w1[4];
+  transpose4(d, w0);
+  transpose4(d + 4, w1);
+  // digit sums of the lane's 8 k, two digits to a word (|sum| <= 2^14)
+  int s[4], s02, s13;
+#pragma unroll
+  for (int l = 0; l < 4; ++l) s[l] = __dp4a((int)w1[l], 0x01010101, __dp4a((int)w0[l], 0x01010101, 0));
+  s02 = s[0] + s[2] * 65536;
+  s13 = s[1] + s[3] * 65536;
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    const int x = __shfl_xor_sync(0xffffffffu, s02, o), y = __shfl_xor_sync(0xffffffffu, s13, o);
+    if (o < glanes) {
+      s02 += x;
+      s13 += y;
+    }
+  }
+  if (!live) return;
+  // 4 lanes per 32-k step, two steps to a half
+  uint8_t* dst = rec + ((hl >> 3) * cols + c0) * 64 + (hl & 3) * 16 + ((hl >> 2) & 1) * 8;
+#pragma unroll
+  for (int l = 0; l < 4; ++l) *reinterpret_cast<uint2*>(dst + l * 64) = make_uint2(w0[l], w1[l]);
+  if (hl % glanes == 0) {
+    const int at = hl / glanes * c8 + c0;
+    float* f = reinterpret_cast<float*>(rec + (size_t)cols * 128);
+    const float f0 = finite ? pow2(e - top) : mx > 0x7f800000u ? __uint_as_float(0x7fc00000u) : INFINITY;
+    // (an infinity sits in the first digit alone)
+    *reinterpret_cast<float2*>(f + at / 2) = make_float2(f0, finite ? f0 * 65536.f : 0.f);
+    const int lo02 = (int)(short)s02, lo13 = (int)(short)s13;
+    *reinterpret_cast<int4*>(reinterpret_cast<int*>(f + ng * c8 / 2) + at) =
+        make_int4(lo02, lo13, (s02 - lo02) >> 16, (s13 - lo13) >> 16);
+  }
+}
+
+// Half a warp per (row, block); grid x over blocks, y over rows.
+__global__ void __launch_bounds__(256) q4g_rows_kernel(const Q4gRows a) {
+  pdl_wait();     // the rows are an earlier kernel's output, and the records
+  pdl_trigger();  // may still be read by the product before this one
+  const int kb = blockIdx.x * 16 + (threadIdx.x >> 4), hl = threadIdx.x & 15;
+  for (int m = blockIdx.y; m < a.M; m += gridDim.y) {
+    const int rb = m / kQgMaxRows, rows = min(kQgMaxRows, a.M - rb * kQgMaxRows);
     float v[8];
-    const int k0 = k8 * 8;
-    if (k0 >= p.K) {  // K is a multiple of 32: a piece is inside or outside
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = 0.f;
-    } else if (p.type == kQgF32) {
-      const float* a = reinterpret_cast<const float*>(p.a) + (size_t)m * p.lda + k0;
-      if (p.vec) {
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(a));
-        const float4 y = __ldcg(reinterpret_cast<const float4*>(a) + 1);
-        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-        v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = __ldcg(a + j);
-      }
-    } else {
-      const unsigned short* a = reinterpret_cast<const unsigned short*>(p.a) + (size_t)m * p.lda + k0;
-      uint32_t u[8];
-      if (p.vec) {
-        const uint4 x = __ldcg(reinterpret_cast<const uint4*>(a));
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) u[j] = (w[j / 2] >> (16 * (j & 1))) & 0xffffu;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) u[j] = __ldcg(a + j);
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        v[j] = p.type == kQgBf16 ? __uint_as_float(u[j] << 16)
-                                 : __half2float(__ushort_as_half((unsigned short)u[j]));
-    }
-    uint32_t l[3][8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (p.limbs == 1)
-        l[0][j] = __float_as_uint(v[j]);
-      else
-        limbs3(v[j], l[0][j], l[1][j], l[2][j]);
-    }
-    const int rb = m / p.mb, r = m % p.mb;
-    const int rows = min(p.mb, p.M - rb * p.mb);
-    uint8_t* base = p.planes + (size_t)rb * p.mb * p.limbs * p.kpad * 2;
-    for (int i = 0; i < p.limbs; ++i) {
-      const uint32_t* s = i == 0 ? l[0] : i == 1 ? l[1] : l[2];
-      uint4 o;
-      o.x = __byte_perm(s[0], s[1], 0x7632);
-      o.y = __byte_perm(s[2], s[3], 0x7632);
-      o.z = __byte_perm(s[4], s[5], 0x7632);
-      o.w = __byte_perm(s[6], s[7], 0x7632);
-      *reinterpret_cast<uint4*>(
-          base + (((size_t)(k0 / 32) * p.limbs + i) * rows + r) * 64 + (k8 & 3) * 16) = o;
-    }
+    load8(a, m, kb * kQgBlockK + 8 * hl, v);
+    uint8_t* rec = a.records + rb * (size_t)a.nkb * qg_record_bytes(kQgMaxRows, a.group) +
+                   (size_t)kb * qg_record_bytes(rows, a.group);
+    convert8(v, a.group, m % kQgMaxRows * kQgDigits, rows * kQgDigits, hl, kb < a.nkb, rec);
   }
 }
 
 // ----------------------------------------------------- streaming kernel --
-// Decode rows.  A warp owns T tiles (T x 16 columns) over its share of the
-// 128-k blocks; the kw warps that share a tile set split K, and their sums
-// are added in k order through shared memory at the end (the same bits on
-// every run).  Each warp streams its own pieces through a private ring of
-// bulk copies: the weight pieces of a block and the same block of the limb
-// planes, one mbarrier per stage and no CTA barrier inside the loop.  The
-// first stages' weights are issued before the previous kernel has finished
-// (nothing writes them); activations and results wait for it.
-constexpr int kQgMaxWarps = 16;
+// Decode rows.  The work is a line of pieces, set by set (a set is T tiles, T x
+// 16 columns, of a weight, or T / 2 of the gate and T / 2 of the up weight)
+// and inside a set by 128-k block.  The CTAs share the sets evenly, and the 16
+// warps of a CTA the pieces of its sets.  A warp streams its pieces through a private ring of
+// bulk copies, one mbarrier per stage and no CTA barrier inside the loop.  A
+// set that lies in one warp's share is finished by that warp; the sums of
+// others meet in shared memory and are added in k order (the same bits on
+// every run).  A CTA has whole sets: a split of the line in the middle of sets,
+// with the last CTA to arrive adding the parts, was balanced to a piece and
+// took 4 us more at every size.
+//   The first stages are issued before the previous kernel has finished
+// (nothing writes the weights); activations and results wait for it.  For few
+// rows the CTA converts the rows into shared memory itself; else their
+// records come with each stage of the ring.
+constexpr int kQgWarps = 16;
 constexpr int kQgMaxStages = 8;
 constexpr size_t kQgSmemMax = 208 * 1024;
 
@@ -190,26 +277,60 @@ __device__ __forceinline__ void store_out(void* p, size_t i, int type, float v) 
     reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
-template <int T, int NB>
-__global__ void __launch_bounds__(kQgMaxWarps* kWarp, T* NB <= 2 ? 2 : 1) q4g_stream_kernel(const Q4gParams p) {
+// n elements in W consecutive parts that differ by one element at most, the
+// longer ones first.
+struct Split {
+  int q, rem;
+  __device__ __forceinline__ Split(int n, int W) : q(n / W), rem(n % W) {}
+  __device__ __forceinline__ int begin(int w) const { return w * q + min(w, rem); }
+  // the part that holds element i
+  __device__ __forceinline__ int of(int i) const {
+    const int head = rem * (q + 1);
+    return i < head ? (int)((unsigned)i / (unsigned)(q + 1))
+                    : rem + (int)((unsigned)(i - head) / (unsigned)max(q, 1));
+  }
+};
+
+// A finished sum v (gated: gate v, up u) of row m, column n.
+__device__ __forceinline__ void finish(const Q4gParams& p, int m, int n, float v, float u) {
+  if (n >= p.w.N) return;
+  if (p.w2) v = act_fn(v, p.act) * u;
+  const size_t at = (size_t)m * p.ldo + n;
+  if (p.accumulate) v += load_out(p.out, at, p.a.type);
+  store_out(p.out, at, p.a.type, v);
+}
+
+// NB: 8-column blocks of digits (2 rows each); G: 32-k steps per group (1, 2, 4).
+template <int T, int NB, int G>
+__global__ void __launch_bounds__(kQgWarps* kWarp, T* NB <= 2 ? 2 : 1)
+    q4g_stream_kernel(const Q4gParams p) {
   extern __shared__ __align__(128) uint8_t dsm[];
-  __shared__ __align__(8) uint64_t s_full[kQgMaxWarps * kQgMaxStages];
+  __shared__ __align__(8) uint64_t s_full[kQgWarps * kQgMaxStages];
+  __shared__ int s_bad;
+  constexpr int kCols = T * kQgTile;  // columns of a set (gate and up)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, t = lane & 3;
-  const int ks = warp % p.kw;
-  const int set = blockIdx.x * p.tw + warp / p.kw;
-  const int n_sets = (q4g_quads(p.w.N) * kQgQuad) / (p.w2 ? T / 2 : T);
-  const int nkb = p.w.nkb, bb = p.w.block_bytes, ng = kQgBlockK / p.w.group;
-  const int row0 = blockIdx.y * p.mb, rows = min(p.mb, p.M - row0);
-  const int L = p.limbs;
-  const int a_bytes = rows * L * 256;
-  const int stage_bytes = T * bb + p.mb * L * 256;
-  const int kb0 = (int)((long long)nkb * ks / p.kw), kb1 = (int)((long long)nkb * (ks + 1) / p.kw);
-  const int n = set < n_sets ? kb1 - kb0 : 0;  // blocks of this warp
-  uint8_t* ring = dsm + (size_t)warp * p.stages * stage_bytes;
+  const int per = p.w2 ? T / 2 : T;  // tiles of each weight in a set
+  const int cols = per * kQgTile;    // result columns of a set
+  const int nkb = p.w.nkb, bb = p.w.block_bytes;
+  constexpr int ng = 4 / G;
+  const int row0 = blockIdx.y * kQgMaxRows, rows = min(kQgMaxRows, p.a.M - row0);
+  const int C = rows * kQgDigits, rc8 = (C + 7) / 8 * 8;
+  const int rec = C * 128 + ng * rc8 * 6;
+  const bool own_a = p.a.records == nullptr;
+  const int stage_bytes = T * bb + (own_a ? 0 : rec);
+  // pieces of the CTA, and of this warp
+  const int set0 = blockIdx.x * p.set_q + min((int)blockIdx.x, p.set_rem);
+  const int sets = p.set_q + ((int)blockIdx.x < p.set_rem);
+  const Split own(sets * nkb, kQgWarps);
+  const int p0 = own.begin(warp), n = own.begin(warp + 1) - p0;
+  float* slots = reinterpret_cast<float*>(dsm + p.a_smem);  // [warps][2][rows][kCols]
+  uint8_t* ring = dsm + p.a_smem + kQgWarps * 2 * rows * kCols * sizeof(float) +
+                  (size_t)warp * p.stages * stage_bytes;
   uint64_t* full = s_full + warp * kQgMaxStages;
 
+  if (threadIdx.x == 0) s_bad = 0;
   if (lane == 0) {
     for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1);
     mbar_fence_init();
@@ -217,43 +338,80 @@ __global__ void __launch_bounds__(kQgMaxWarps* kWarp, T* NB <= 2 ? 2 : 1) q4g_st
   __syncwarp();
   pdl_trigger();
 
-  // the pieces of tiles set * T .. (gated: T / 2 of the gate, then of the up)
-  const int per = p.w2 ? T / 2 : T;
-  const int tile0 = set * per;
-  const size_t w_off = ((size_t)(tile0 / kQgQuad) * nkb * kQgQuad + tile0 % kQgQuad) * bb;
-  const uint8_t* a_src = p.planes + (size_t)row0 * L * nkb * 256;
-  auto issue_w = [&](int i) {
-    uint8_t* st = ring + (size_t)(i % p.stages) * stage_bytes;
-    uint64_t* bar = &full[i % p.stages];
-    const size_t off = w_off + (size_t)(kb0 + i) * kQgQuad * bb;
-    mbar_expect_tx(bar, T * bb + a_bytes);
-    bulk_g2s(st, p.w.w + off, per * bb, bar);
-    if (p.w2) bulk_g2s(st + per * bb, p.w2 + off, per * bb, bar);
+  // the next piece to copy
+  const int first_set = p0 / nkb;
+  int i_set = set0 + first_set, i_kb = p0 - first_set * nkb;
+  const int i_set0 = i_set, i_kb0 = i_kb;
+  size_t i_off = 0;
+  auto seek = [&]() {
+    const int tile = i_set * per;
+    i_off = (((size_t)(tile / kQgQuad) * nkb + i_kb) * kQgQuad + tile % kQgQuad) * bb;
   };
-  auto issue_a = [&](int i) {
-    bulk_g2s(ring + (size_t)(i % p.stages) * stage_bytes + T * bb, a_src + (size_t)(kb0 + i) * a_bytes,
-             a_bytes, &full[i % p.stages]);
+  seek();
+  const uint8_t* a_src =
+      own_a ? nullptr
+            : p.a.records + (size_t)blockIdx.y * nkb * qg_record_bytes(kQgMaxRows, p.w.group);
+  auto issue_w = [&](int slot) {
+    uint8_t* st = ring + slot * stage_bytes;
+    mbar_expect_tx(&full[slot], stage_bytes);
+    bulk_g2s(st, p.w.w + i_off, per * bb, &full[slot]);
+    if (p.w2) bulk_g2s(st + per * bb, p.w2 + i_off, per * bb, &full[slot]);
+  };
+  auto issue_a = [&](int slot, int kb) {
+    bulk_g2s(ring + slot * stage_bytes + T * bb, a_src + (size_t)kb * rec, rec, &full[slot]);
+  };
+  auto advance = [&]() {
+    i_off += kQgQuad * bb;
+    if (++i_kb == nkb) {
+      i_kb = 0;
+      ++i_set;
+      seek();
+    }
   };
   const int first = min(n, p.stages);
   if (lane == 0)
-    for (int i = 0; i < first; ++i) issue_w(i);
+    for (int i = 0; i < first; ++i) {
+      issue_w(i);
+      advance();
+    }
   pdl_wait();
-  if (lane == 0)
-    for (int i = 0; i < first; ++i) issue_a(i);
+  int set = i_set0, kb = i_kb0;
+  if (own_a) {
+    // two (row, block) items per warp and round, the next round's loads first
+    const int items = rows * nkb, hl = lane & 15;
+    int it = warp * 2 + (lane >> 4);
+    float v[8], nx[8];
+    load8(p.a, row0 + it / nkb, it < items ? it % nkb * kQgBlockK + 8 * hl : p.a.K, v);
+    for (; __any_sync(0xffffffffu, it < items); it += 2 * kQgWarps) {
+      const int nt = it + 2 * kQgWarps;
+      load8(p.a, row0 + nt / nkb, nt < items ? nt % nkb * kQgBlockK + 8 * hl : p.a.K, nx);
+      convert8(v, p.w.group, it / nkb * kQgDigits, C, hl, it < items, dsm + (size_t)(it % nkb) * rec);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = nx[j];
+    }
+    __syncthreads();
+  } else if (lane == 0) {
+    for (int i = 0; i < first; ++i) issue_a(i, (kb + i) % nkb);
+  }
 
-  float acc[T][NB][4];
+  float acc[T][NB][2];  // columns r and r + 8 of a tile
 #pragma unroll
   for (int i = 0; i < T; ++i)
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][b][j] = 0.f;
+    for (int b = 0; b < NB; ++b) acc[i][b][0] = acc[i][b][1] = 0.f;
+  // a row's digits are with lanes t = 0, 1 (row 0 of a column block) or 2, 3 (row 1)
+  auto row_sums = [&](int j, int b, float& lo, float& hi) {
+    lo = acc[j][b][0] + __shfl_xor_sync(0xffffffffu, acc[j][b][0], 1);
+    hi = acc[j][b][1] + __shfl_xor_sync(0xffffffffu, acc[j][b][1], 1);
+  };
 
-  const int flush_mask = p.w.group / 32 - 1;  // a group ends after 32-k step h if (h & mask) == mask
+  const uint32_t dsm_s = smem_u32(dsm), ring_s = smem_u32(ring);
   bool ok = true;
+  int slot = 0;
+  uint32_t phase = 0;
+  int begun = kb;  // block of the set that this warp's sum starts at
   for (int i = 0; i < n; ++i) {
-    const int slot = i % p.stages;
-    if (!mbar_wait(&full[slot], (i / p.stages) & 1)) {
+    if (!mbar_wait(&full[slot], phase)) {
       if (lane == 0) atomicOr(p.err, kErrWaitTimeout);
       // let the other copies land before the CTA can exit
       for (int j = i + 1; j < min(n, i + p.stages); ++j)
@@ -261,80 +419,79 @@ __global__ void __launch_bounds__(kQgMaxWarps* kWarp, T* NB <= 2 ? 2 : 1) q4g_st
       ok = false;
       break;
     }
-    const uint8_t* st = ring + (size_t)slot * stage_bytes;
-    const uint8_t* sa = st + T * bb;
-    float c[T][NB][4];
-    uint32_t bias[T][2];
+    const uint32_t st = ring_s + slot * stage_bytes;
+    const uint32_t sa = own_a ? dsm_s + kb * rec : st + T * bb;
+    const uint32_t fac = sa + C * 128 + 4 * t, sums = sa + C * 128 + ng * rc8 * 2 + 8 * t;
+    const uint32_t wl = st + lane * 16;
+    const uint32_t sc = st + kQgNibbles + r * 4;
+    int c[T][NB][4];
+    int ci[NB][4];  // -z times the group's digit sums (column r + 8 counts 16-fold)
+    uint2 sd[NB];
+    float f[NB];
 #pragma unroll
     for (int q = 0; q < 2; ++q) {  // 64-k halves
+      uint4 bv[NB];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        bv[b] = make_uint4(0u, 0u, 0u, 0u);
+        if (b * 8 + r < C) bv[b] = lds128(sa + r * 64 + t * 16 + (q * C + b * 8) * 64);
+      }
       uint4 wv[T];
 #pragma unroll
-      for (int j = 0; j < T; ++j)
-        wv[j] = lds_u4(reinterpret_cast<const uint4*>(st + j * bb + q * 512) + lane);
+      for (int j = 0; j < T; ++j) wv[j] = lds128(wl + j * bb + q * 512);
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {  // 32-k steps
-        const int h = 2 * q + hh;
-        const int grp = h / (flush_mask + 1);
-        if ((h & flush_mask) == 0) {  // a group begins
-#pragma unroll
-          for (int j = 0; j < T; ++j) {
-            uint32_t lo = 0x43084308u, hi = 0x43084308u;  // 128 + 8
-            if (p.w.zeros) {
-              const uint32_t z = *reinterpret_cast<const uint16_t*>(st + j * bb + kQgNibbles +
-                                                                    ng * 32 + (grp * 8 + r) * 2);
-              lo = (0x4300u | (z & 0xffu)) * 0x10001u;
-              hi = (0x4300u | (z >> 8)) * 0x10001u;
-            }
-            bias[j][0] = lo;
-            bias[j][1] = hi;
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) c[j][b][e] = 0.f;
-          }
-        }
-        uint32_t a[T][2][4];
-#pragma unroll
-        for (int j = 0; j < T; ++j)
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            const uint32_t w = hh == 0 ? (s == 0 ? wv[j].x : wv[j].y) : (s == 0 ? wv[j].z : wv[j].w);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t v = ((w >> (4 * e)) & 0x000F000Fu) | 0x43004300u;
-              asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(a[j][s][e]) : "r"(v), "r"(bias[j][e & 1]));
-            }
-          }
-        for (int l = 0; l < L; ++l) {
-          uint4 bv[NB];
+        const int h = 2 * q + hh, grp = h / G;
+        if (h % G == 0) {  // a group begins
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
-            const int m = b * 8 + r;
-            bv[b] = make_uint4(0u, 0u, 0u, 0u);
-            if (m < rows)
-              bv[b] = lds_u4(reinterpret_cast<const uint4*>(sa + ((h * L + l) * rows + m) * 64) + t);
+            f[b] = 0.f;
+            sd[b] = make_uint2(0u, 0u);
+            if (b * 8 < C) {
+              f[b] = __uint_as_float(lds32(fac + (grp * rc8 / 2 + b * 4) * 4));
+              sd[b] = lds64(sums + (grp * rc8 + b * 8) * 4);
+            }
+            ci[b][0] = -8 * (int)sd[b].x;
+            ci[b][1] = -8 * (int)sd[b].y;
+            ci[b][2] = -128 * (int)sd[b].x;
+            ci[b][3] = -128 * (int)sd[b].y;
           }
+        }
 #pragma unroll
-          for (int j = 0; j < T; ++j)
+        for (int j = 0; j < T; ++j) {
+          if (h % G == 0 && p.w.zeros) {
+            const uint32_t z = lds16(st + j * bb + kQgNibbles + ng * 32 + (grp * 8 + r) * 2);
+            const int zl = -(int)(z & 0xffu), zh = -16 * (int)(z >> 8);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-              mma_bf16_16816(c[j][b], a[j][0], bv[b].x, bv[b].y);
-              mma_bf16_16816(c[j][b], a[j][1], bv[b].z, bv[b].w);
+              ci[b][0] = zl * (int)sd[b].x;
+              ci[b][1] = zl * (int)sd[b].y;
+              ci[b][2] = zh * (int)sd[b].x;
+              ci[b][3] = zh * (int)sd[b].y;
             }
+          }
+          const uint32_t x0 = hh == 0 ? wv[j].x : wv[j].z, x1 = hh == 0 ? wv[j].y : wv[j].w;
+          const uint32_t a0 = x0 & 0x0F0F0F0Fu, a1 = x0 & 0xF0F0F0F0u;
+          const uint32_t a2 = x1 & 0x0F0F0F0Fu, a3 = x1 & 0xF0F0F0F0u;
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            const uint32_t b0 = hh == 0 ? bv[b].x : bv[b].z, b1 = hh == 0 ? bv[b].y : bv[b].w;
+            if (h % G == 0)
+              mma_u8s8_16832(c[j][b], a0, a1, a2, a3, b0, b1, ci[b]);
+            else
+              mma_u8s8_16832(c[j][b], a0, a1, a2, a3, b0, b1, c[j][b]);
+          }
         }
-        if ((h & flush_mask) == flush_mask) {  // it ends
+        if (h % G == G - 1) {  // it ends: two digits in one integer (|sum| < 2^30)
 #pragma unroll
           for (int j = 0; j < T; ++j) {
-            const uint32_t s2 = *reinterpret_cast<const uint32_t*>(st + j * bb + kQgNibbles +
-                                                                   (grp * 8 + r) * 4);
+            const uint32_t s2 = lds32(sc + j * bb + grp * 32);
             const float lo = u16_scale(s2 & 0xffffu, p.w.bf_scale);
-            const float hi = u16_scale(s2 >> 16, p.w.bf_scale);
+            const float hi = 0.0625f * u16_scale(s2 >> 16, p.w.bf_scale);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-              acc[j][b][0] = fmaf(lo, c[j][b][0], acc[j][b][0]);
-              acc[j][b][1] = fmaf(lo, c[j][b][1], acc[j][b][1]);
-              acc[j][b][2] = fmaf(hi, c[j][b][2], acc[j][b][2]);
-              acc[j][b][3] = fmaf(hi, c[j][b][3], acc[j][b][3]);
+              acc[j][b][0] = fmaf(lo * f[b], (float)(c[j][b][0] + 256 * c[j][b][1]), acc[j][b][0]);
+              acc[j][b][1] = fmaf(hi * f[b], (float)(c[j][b][2] + 256 * c[j][b][3]), acc[j][b][1]);
             }
           }
         }
@@ -342,96 +499,158 @@ __global__ void __launch_bounds__(kQgMaxWarps* kWarp, T* NB <= 2 ? 2 : 1) q4g_st
     }
     __syncwarp();  // every lane has read the stage
     if (lane == 0 && i + p.stages < n) {
-      issue_w(i + p.stages);
-      issue_a(i + p.stages);
+      issue_w(slot);
+      if (!own_a) issue_a(slot, i_kb);
+      advance();
     }
-  }
-
-  // sums over the kw warps of a tile set, in k order; columns fastest
-  constexpr int kCols = T * kQgTile, kLd = kCols + 4;
-  __syncthreads();  // the rings are free
-  float* red = reinterpret_cast<float*>(dsm);
-  if (ok && n > 0) {
-    float* mine = red + (size_t)warp * (NB * 8) * kLd;
+    if (++slot == p.stages) {
+      slot = 0;
+      phase ^= 1;
+    }
+    if (++kb == nkb || i + 1 == n) {  // the warp's share of this set is complete
+      if (begun == 0 && kb == nkb) {  // all of it
 #pragma unroll
-    for (int j = 0; j < T; ++j)
+        for (int j = 0; j < T; ++j)
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        float* d = mine + (b * 8 + 2 * t) * kLd + j * kQgTile + r;
-        d[0] = acc[j][b][0];
-        d[kLd] = acc[j][b][1];
-        d[8] = acc[j][b][2];
-        d[kLd + 8] = acc[j][b][3];
+          for (int b = 0; b < NB; ++b) {
+            float lo, hi, ulo = 0.f, uhi = 0.f;
+            if (p.w2 && j >= T / 2) break;
+            row_sums(j, b, lo, hi);
+            if (p.w2) row_sums((j + T / 2) % T, b, ulo, uhi);
+            const int m = 2 * b + (t >> 1);
+            if (!(t & 1) && m < rows) {
+              finish(p, row0 + m, set * cols + j * kQgTile + r, lo, ulo);
+              finish(p, row0 + m, set * cols + j * kQgTile + r + 8, hi, uhi);
+            }
+          }
+      } else {
+        float* d = slots + (size_t)(warp * 2 + (set != i_set0)) * rows * kCols;
+#pragma unroll
+        for (int j = 0; j < T; ++j)
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            float lo, hi;
+            row_sums(j, b, lo, hi);
+            const int m = 2 * b + (t >> 1);
+            if (!(t & 1) && m < rows) {
+              d[m * kCols + j * kQgTile + r] = lo;
+              d[m * kCols + j * kQgTile + r + 8] = hi;
+            }
+          }
       }
-  }
-  if (__syncthreads_or(!ok)) return;  // nothing is written after a wait that ran out
-  const int live = min(p.kw, nkb);    // warps past that had no blocks
-  const int cols = per * kQgTile;     // result columns of a tile set
-  for (int i = threadIdx.x; i < p.tw * rows * cols; i += blockDim.x) {
-    const int col = i % cols, m = i / cols % rows, ts = i / (cols * rows);
-    const int set_i = blockIdx.x * p.tw + ts;
-    const int nn = set_i * cols + col;
-    if (set_i >= n_sets || nn >= p.w.N) continue;
-    const float* src = red + ((size_t)ts * p.kw * (NB * 8) + m) * kLd + col;
-    float v = 0.f, u = 0.f;
-    for (int k = 0; k < p.kw; ++k) {
-      // block ranges nkb k / kw .. nkb (k + 1) / kw: empty where kw > nkb
-      if (live < p.kw && (long long)nkb * k / p.kw == (long long)nkb * (k + 1) / p.kw) continue;
-      v += src[(size_t)k * (NB * 8) * kLd];
-      if (p.w2) u += src[(size_t)k * (NB * 8) * kLd + cols];
+#pragma unroll
+      for (int j = 0; j < T; ++j)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc[j][b][0] = acc[j][b][1] = 0.f;
+      if (kb == nkb) {
+        kb = 0;
+        ++set;
+      }
+      begun = kb;
     }
-    if (p.w2) v = act_fn(v, p.act) * u;
-    const size_t at = (size_t)(row0 + m) * p.ldo + nn;
-    if (p.accumulate) v += load_out(p.out, at, p.type);
-    store_out(p.out, at, p.type, v);
+  }
+  if (!ok) s_bad = 1;
+  __syncthreads();
+  if (s_bad) return;  // nothing more is written after a wait that ran out
+
+  // sets that no single warp covers: sums over the warps in k order
+  const int cl = 31 - __clz(cols);
+  for (int i = threadIdx.x; i < sets * rows << cl; i += blockDim.x) {
+    const int col = i & (cols - 1), sm = i >> cl, s = rows == 1 ? sm : sm / rows, m = sm - s * rows;
+    const int q0 = s * nkb, wa = own.of(q0), wb = own.of(q0 + nkb - 1);
+    if (wa == wb) continue;
+    // a warp's first set sits in its first slot, its last one in the second
+    float v = 0.f, u = 0.f;
+#pragma unroll 4
+    for (int w = wa; w <= wb; ++w) {
+      const float* d = slots + ((w * 2 + (own.begin(w) < q0)) * rows + m) * kCols + col;
+      v += d[0];
+      if (p.w2) u += d[cols];
+    }
+    finish(p, row0 + m, (set0 + s) * cols + col, v, u);
   }
 }
 
-template <int T, int NB>
-cudaError_t launch_stream_t(const Q4gParams& p0, int sm_count, cudaStream_t s) {
-  Q4gParams p = p0;
-  const int per = p.w2 ? T / 2 : T;
-  const int sets = q4g_quads(p.w.N) * kQgQuad / per;
-  const int row_blocks = (p.M + p.mb - 1) / p.mb;
-  // 16 warps, fewer where three stages of theirs would not fit; as many tile
-  // sets as still leave two CTAs for each SM, the rest of the warps split K
-  const size_t stage = (size_t)T * p.w.block_bytes + (size_t)p.mb * p.limbs * 256;
-  int warps = kQgMaxWarps;
-  while (warps > 2 && 3 * stage * warps > kQgSmemMax) warps /= 2;
-  int tw = warps;
-  while (tw > 1 && (long long)(sets + tw - 1) / tw * row_blocks < 2LL * sm_count) tw /= 2;
-  const int kw = warps / tw;
-  p.tw = tw;
-  p.kw = kw;
-  size_t budget = kQgSmemMax / 2;  // two CTAs per SM where three stages fit
-  if (3 * stage * warps > budget) budget = kQgSmemMax;
-  int st = (int)(budget / (stage * warps));
-  const int longest = (p.w.nkb + kw - 1) / kw;
+struct StreamPlan {
+  int T, NB, ctas, stages, sets;
+  size_t a_smem, smem;
+};
+
+StreamPlan plan_stream(const Q4gParams& p, int sm_count) {
+  StreamPlan o{};
+  const int rows = p.a.M < kQgMaxRows ? p.a.M : kQgMaxRows;
+  const int row_blocks = (p.a.M + kQgMaxRows - 1) / kQgMaxRows;
+  o.NB = (rows + 1) / 2;
+  // four tiles to a set share a block's loads and loop (one row, K 2560, N
+  // 20480: 7.6 us, with two 8.6 us) where the GPU still gets a set per SM;
+  // fewer columns fill it better with two (N 2560: 4.5 us, with four 4.6 us).
+  // From five rows on four tiles' sums do not fit the registers.
+  const int quads = q4g_quads(p.w.N) * (p.w2 ? 2 : 1);
+  o.T = o.NB <= 2 && quads >= sm_count ? 4 : 2;
+  o.sets = quads * kQgQuad / o.T;
+  // rows x blocks that 16 warps convert in three rounds (about 1 us); more
+  // come converted (2 us, mostly the launch, at any size)
+  const size_t rec = (size_t)qg_record_bytes(rows, p.w.group);
+  const size_t a_all = p.w.nkb * rec;
+  o.a_smem = row_blocks == 1 && rows * p.w.nkb <= 6 * kQgWarps && a_all <= 64 * 1024 ? a_all : 0;
+  const size_t stage = (size_t)o.T * p.w.block_bytes + (o.a_smem ? 0 : rec);
+  const size_t fixed = o.a_smem + (size_t)kQgWarps * 2 * rows * o.T * kQgTile * sizeof(float);
+  // small sets run two CTAs to an SM (64 registers)
+  const bool two = o.T * o.NB <= 2 && fixed + 2 * stage * kQgWarps <= kQgSmemMax / 2;
+  o.ctas = sm_count * (two ? 2 : 1);
+  if (o.sets < o.ctas) o.ctas = o.sets;
+  int st = (int)(((two ? kQgSmemMax / 2 : kQgSmemMax) - fixed) / (stage * kQgWarps));
+  const long long longest =
+      ((long long)(o.sets + o.ctas - 1) / o.ctas * p.w.nkb + kQgWarps - 1) / kQgWarps;
   st = st > kQgMaxStages ? kQgMaxStages : st;
-  st = st > longest ? longest : st;
-  if (st < 1) return cudaErrorInvalidConfiguration;
-  p.stages = st;
-  size_t smem = (size_t)st * stage * warps;
-  const size_t red = (size_t)warps * NB * 8 * (T * kQgTile + 4) * sizeof(float);
-  if (red > smem) smem = red;
-  if (smem > kQgSmemMax) return cudaErrorInvalidConfiguration;
+  st = st > longest ? (int)longest : st;
+  o.stages = st;
+  o.smem = fixed + (size_t)st * stage * kQgWarps;
+  return o;
+}
+
+template <int T, int NB, int G>
+cudaError_t launch_stream_t(const Q4gParams& p0, const StreamPlan& o, cudaStream_t s) {
+  Q4gParams p = p0;
+  p.stages = o.stages;
+  p.a_smem = (int)o.a_smem;
+  p.set_q = o.sets / o.ctas;
+  p.set_rem = o.sets % o.ctas;
+  if (o.stages < 1 || o.smem > kQgSmemMax || !p.a.records != (o.a_smem > 0))
+    return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((sets + tw - 1) / tw, row_blocks, 1);
-  cfg.blockDim = dim3(warps * kWarp);
-  cfg.dynamicSmemBytes = smem;
+  cfg.gridDim = dim3(o.ctas, (p.a.M + kQgMaxRows - 1) / kQgMaxRows, 1);
+  cfg.blockDim = dim3(kQgWarps * kWarp);
+  cfg.dynamicSmemBytes = o.smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, q4g_stream_kernel<T, NB>, p);
+  return cudaLaunchKernelEx(&cfg, q4g_stream_kernel<T, NB, G>, p);
 }
 
 template <int T, int NB>
+cudaError_t launch_stream_g(const Q4gParams& p, const StreamPlan& o, cudaStream_t s) {
+  switch (p.w.group) {
+    case 32: return launch_stream_t<T, NB, 1>(p, o, s);
+    case 64: return launch_stream_t<T, NB, 2>(p, o, s);
+    default: return launch_stream_t<T, NB, 4>(p, o, s);
+  }
+}
+
+template <int T, int NB, int G>
 cudaError_t prepare_t() {
-  return cudaFuncSetAttribute(q4g_stream_kernel<T, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              (int)kQgSmemMax);
+  return cudaFuncSetAttribute(q4g_stream_kernel<T, NB, G>,
+                              cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kQgSmemMax);
+}
+template <int T, int NB>
+cudaError_t prepare_g() {
+  cudaError_t e = prepare_t<T, NB, 1>();
+  if (e == cudaSuccess) e = prepare_t<T, NB, 2>();
+  if (e == cudaSuccess) e = prepare_t<T, NB, 4>();
+  return e;
 }
 
 }  // namespace
@@ -445,35 +664,48 @@ cudaError_t launch_q4g_repack(uint8_t* out, const Q4gView& v, const uint8_t* src
   return cudaGetLastError();
 }
 
-cudaError_t launch_q4g_planes(const Q4gPlanes& p, cudaStream_t s) {
-  const int k8 = p.kpad / 8;
-  const int threads = k8 < 256 ? (k8 + 31) / 32 * 32 : 256;
+size_t q4g_records_bytes(const Q4gRows& r) {
+  return (size_t)((r.M + kQgMaxRows - 1) / kQgMaxRows) * r.nkb *
+         qg_record_bytes(kQgMaxRows, r.group);
+}
+
+cudaError_t launch_q4g_rows(const Q4gRows& r, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((k8 + threads - 1) / threads, p.M < 65535 ? p.M : 65535, 1);
-  cfg.blockDim = dim3(threads);
+  cfg.gridDim = dim3((r.nkb + 15) / 16, r.M < 65535 ? r.M : 65535, 1);
+  cfg.blockDim = dim3(256);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, q4g_planes_kernel, p);
+  return cudaLaunchKernelEx(&cfg, q4g_rows_kernel, r);
 }
 
-cudaError_t launch_q4g_stream(const Q4gParams& p, int T, int NB, int sm_count, cudaStream_t s) {
-  if (p.mb > NB * 8 || p.mb <= 0 || (p.w2 && T < 2)) return cudaErrorInvalidValue;
-  if (NB == 1 && T == 1) return launch_stream_t<1, 1>(p, sm_count, s);
-  if (NB == 1 && T == 2) return launch_stream_t<2, 1>(p, sm_count, s);
-  if (NB == 1 && T == 4) return launch_stream_t<4, 1>(p, sm_count, s);
-  if (NB == 2 && T == 2) return launch_stream_t<2, 2>(p, sm_count, s);
+bool q4g_stream_converts(const Q4gParams& p, int sm_count) {
+  return plan_stream(p, sm_count).a_smem > 0;
+}
+
+cudaError_t launch_q4g_stream(const Q4gParams& p, int sm_count, cudaStream_t s) {
+  const StreamPlan o = plan_stream(p, sm_count);
+  switch (o.T * 8 + o.NB) {  // the plan's own shape, or nothing
+    case 2 * 8 + 1: return launch_stream_g<2, 1>(p, o, s);
+    case 4 * 8 + 1: return launch_stream_g<4, 1>(p, o, s);
+    case 4 * 8 + 2: return launch_stream_g<4, 2>(p, o, s);
+    case 2 * 8 + 2: return launch_stream_g<2, 2>(p, o, s);
+    case 2 * 8 + 3: return launch_stream_g<2, 3>(p, o, s);
+    case 2 * 8 + 4: return launch_stream_g<2, 4>(p, o, s);
+  }
   return cudaErrorInvalidValue;
 }
 
 cudaError_t prepare_q4g() {
-  cudaError_t e = prepare_t<1, 1>();
-  if (e == cudaSuccess) e = prepare_t<2, 1>();
-  if (e == cudaSuccess) e = prepare_t<4, 1>();
-  if (e == cudaSuccess) e = prepare_t<2, 2>();
+  cudaError_t e = prepare_g<2, 1>();
+  if (e == cudaSuccess) e = prepare_g<4, 1>();
+  if (e == cudaSuccess) e = prepare_g<4, 2>();
+  if (e == cudaSuccess) e = prepare_g<2, 2>();
+  if (e == cudaSuccess) e = prepare_g<2, 3>();
+  if (e == cudaSuccess) e = prepare_g<2, 4>();
   return e;
 }
 

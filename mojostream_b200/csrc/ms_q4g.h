@@ -16,10 +16,11 @@
 //   bits  4- 7 / 20-23 : column r + 8, k + 0 / k + 1
 //   bits  8-11 / 24-27 : column r    , k + 2 / k + 3
 //   bits 12-15 / 28-31 : column r + 8, k + 2 / k + 3
-// which is the A operand (16 columns x 16 k) of one mma.m16n8k16 with the k of
-// the MMA permuted so that a lane's share of an activation row is 8 values in
-// a row.  Blocks past K and columns past N hold nibble 8, zero point 8 and
-// scale 0.
+// so that masking a word with 0x0F0F0F0F gives four bytes q of column r and
+// masking it with 0xF0F0F0F0 four bytes 16 q of column r + 8: half of the A
+// operand (16 columns x 32 k) of an integer mma.m16n8k32 whose k are permuted
+// so that a lane's share of an activation row is 8 values in a row.  Blocks
+// past K and columns past N hold nibble 8, zero point 8 and scale 0.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -49,42 +50,54 @@ __host__ __device__ inline int q4g_quads(int N) { return (N + 63) / 64; }
 
 // Element types of activations and results (MS_F32, MS_BF16, MS_F16).
 enum QgType : int { kQgF32 = 0, kQgBf16 = 1, kQgF16 = 2 };
-// bfloat16 limbs that hold a value of a type exactly: 24 = 8 + 8 + 8 bits,
-// 11 = 8 + 3 bits.
-__host__ __device__ inline int qg_limbs(int type) {
-  return type == kQgF32 ? 3 : type == kQgF16 ? 2 : 1;
+
+// Decode rows (streaming kernel): activations as four signed 8-bit digits.
+// For a row and a group of k with 2^e <= max |a| < 2^(e + 1),
+// q = rint(a 2^(29 - e)) = sum_l d_l 256^l: a value within 2^6 (fp32) or 2^21
+// (bfloat16) of its group's largest is held exactly, any other to 2^-30 of the
+// largest.  A digit of a row is a column of the MMA: C = 4 rows, padded to a
+// multiple of 8.  Record of a 128-k block:
+//   2 x [C] x 64 bytes   the 64-k halves of each column, in fragment order
+//   [128 / g][C8 / 2] float  factors 2^(e - 29), 2^(e - 13) of a row's lower
+//                            and upper two digits
+//   [128 / g][C8] int        sums of the group's digits
+constexpr int kQgMaxRows = 8;
+constexpr int kQgDigits = 4;
+__host__ __device__ inline int qg_record_bytes(int rows, int group) {
+  return rows * kQgDigits * 128 + (kQgBlockK / group) * ((rows + 1) / 2 * 8) * 6;
 }
+
+struct Q4gRows {
+  const void* a;
+  long long lda;
+  int type, M, K, nkb, group;
+  int vec;           // rows start on 16-byte boundaries
+  uint8_t* records;  // [row block of 8][128-k block]
+};
 
 struct Q4gParams {
   Q4gView w;         // the weight, or the gate
   const uint8_t* w2; // gated: the up weight (same shape and groups), else null
-  // activations as bfloat16 limb planes, row blocks of `mb` rows:
-  // [row block][k / 32][limb][row in block][32 k], k padded to 128
-  const uint8_t* planes;
-  int limbs, M, mb;
+  Q4gRows a;         // records null: the CTAs convert the rows themselves
   void* out;
   long long ldo;
-  int type;          // of out
   int accumulate;
   int act;           // gated: 0 SiLU, 1 tanh-GELU
   int* err;
-  // launch shape of the streaming kernel
-  int kw, tw, stages;
-};
-
-// Activation rows (any type and stride) to limb planes.
-struct Q4gPlanes {
-  const void* a;
-  long long lda;
-  int type, M, K, kpad, mb, limbs;
-  int vec;           // rows start on 16-byte boundaries
-  uint8_t* planes;
+  // launch shape of the streaming kernel: ring stages, bytes of converted
+  // rows, sets of a CTA (one more in the first set_rem CTAs)
+  int stages, a_smem, set_q, set_rem;
 };
 
 cudaError_t launch_q4g_repack(uint8_t* out, const Q4gView& v, const uint8_t* src, const void* scales,
                               const uint8_t* zeros, int* bad, cudaStream_t s);
-cudaError_t launch_q4g_planes(const Q4gPlanes& p, cudaStream_t s);
-cudaError_t launch_q4g_stream(const Q4gParams& p, int T, int NB, int sm_count, cudaStream_t s);
+// Rows to records, blocks of kQgMaxRows rows.
+cudaError_t launch_q4g_rows(const Q4gRows& r, cudaStream_t s);
+size_t q4g_records_bytes(const Q4gRows& r);
+// Any number of rows, kQgMaxRows at a time.  q4g_stream_converts: the launch
+// needs no records.
+bool q4g_stream_converts(const Q4gParams& p, int sm_count);
+cudaError_t launch_q4g_stream(const Q4gParams& p, int sm_count, cudaStream_t s);
 cudaError_t prepare_q4g();
 
 }  // namespace ms

@@ -1,12 +1,20 @@
 """Products with group-scaled 4-bit weights and the gated half on them
 (ms_q4g_gemm, ms_q4g_gated) against their definition in 64 bits.
 
-Bound.  Every product a * (q - z) is exact; an MMA of 16 k adds to an fp32
-accumulator with an error of at most 4 u (u = 2^-24: alignment of the addends
-and the final rounding) of the magnitudes that it adds, a group of g values
-takes g / 16 MMAs per limb, and the K / g group sums and at most 16 partial
-sums are added with one rounding each, so
-    |C - exact| <= (4 limbs g / 16 + K / g + 20) u sum_k |a w|  + half a step of the type.
+Bounds, with u = 2^-24 and S = sum_k |a w|; the larger of the two holds for
+any number of rows.
+  Integer digits (decode rows).  A value is held to half a step of its group's
+scale: 2^-30 (fp32) or 2^-22 (16-bit types) of the group's largest value, at
+least 2^-120.  Group sums of digits are exact; per digit the K / g groups are
+scaled and added in fp32, the digits of a value add up to at most 2 |a| in
+magnitude, and scale, factor, up to 16 + 8 partial sums and the digits cost
+one rounding each:  2 (K / g + 32) u S.
+  bfloat16 limbs (more rows).  Every product is exact; an MMA of 16 k adds to
+an fp32 accumulator with an error of at most 4 u (alignment of the addends and
+the final rounding) of the magnitudes that it adds, a group takes g / 16 MMAs
+per limb, and the group and partial sums one rounding each:
+(4 limbs g / 16 + K / g + 20) u S.
+  Then half a step of the result's type.
 """
 import math
 
@@ -50,12 +58,26 @@ def dense(q, s, z, g):
     return (v - (8.0 if z is None else z[group].astype(np.float64))) * s.astype(np.float64)[group]
 
 
-def bound(torch, dtype, g, K, mag, exact):
-    name = str(dtype).replace("torch.", "")
-    tol = (4 * LIMBS[name] * g / 16 + K / g + 20) * U * mag
-    # half a step of the result's type (and of its smallest step near zero)
+def sums_bound(name, g, a64, wd):
+    """Bound of |sum - exact| before the result is rounded."""
+    K = wd.shape[0]
+    mag = np.abs(a64) @ np.abs(wd)
+    steps = max(4 * LIMBS[name] * g / 16 + K / g + 20, 2 * (K / g + 32))
+    half = 2.0 ** -30 if name == "float32" else 2.0 ** -22
+    top = np.abs(a64).reshape(len(a64), K // g, g).max(2)
+    per_group = np.abs(wd).reshape(K // g, g, -1).sum(1)
+    return steps * U * mag + np.maximum(half * top, 2.0 ** -120) @ per_group
+
+
+def rounded(torch, dtype, tol, exact):
+    """A bound after rounding to dtype (half a step, or of its smallest step near zero)."""
     half = torch.finfo(dtype).eps / 2
     return tol * (1 + half) + half * np.abs(exact) + torch.finfo(dtype).smallest_normal * half
+
+
+def bound(torch, dtype, g, a64, wd, exact, c0=0.0):
+    tol = sums_bound(str(dtype).replace("torch.", ""), g, a64, wd) + U * (np.abs(exact) + np.abs(c0))
+    return rounded(torch, dtype, tol, exact)
 
 
 def rows(torch, rng, M, K, pad, dtype):
@@ -82,9 +104,8 @@ def check(torch, ctx, M, K, N, g, zeros, dtype, pad, seed=0, accumulate=False):
     assert out is c
     a64, wd = a.double().cpu().numpy(), dense(q, s, z, g)
     exact = a64 @ wd + c0
-    mag = np.abs(a64) @ np.abs(wd) + np.abs(c0)
-    err = np.abs(c.double().cpu().numpy() - exact)
-    assert (err <= bound(torch, dtype, g, K, mag, exact)).all(), float((err / mag).max())
+    err, tol = np.abs(c.double().cpu().numpy() - exact), bound(torch, dtype, g, a64, wd, exact, c0)
+    assert (err <= tol).all(), float((err / tol).max())
     # nothing beside the result is touched
     assert (buf[M] == 7).all() and (buf[:, N:] == 7).all()
     w.close()
@@ -136,8 +157,8 @@ def test_bf16_scales_and_device_sources(ctx, torch_cuda, M):
     c = torch.empty((M, N), device="cuda")
     w.gemm(a, c)
     a64, wd = a.double().cpu().numpy(), dense(q, sb.double().cpu().numpy(), z, g)
-    exact, mag = a64 @ wd, np.abs(a64) @ np.abs(wd)
-    assert (np.abs(c.double().cpu().numpy() - exact) <= bound(torch, torch.float32, g, K, mag, exact)).all()
+    exact = a64 @ wd
+    assert (np.abs(c.double().cpu().numpy() - exact) <= bound(torch, torch.float32, g, a64, wd, exact)).all()
     assert w.nbytes >= K * N // 2
 
 
@@ -169,8 +190,7 @@ def test_infinities_and_nans_stay_in_their_rows(ctx, torch_cuda, dtype, M):
     assert np.isnan(got[3]).all()
     assert not np.isfinite(got[4]).any()
     fine = [r for r in range(M) if r not in (1, 3, 4)]
-    mag = np.abs(a64[fine]) @ np.abs(wd)
-    assert (np.abs(got[fine] - exact[fine]) <= bound(torch, dt, g, K, mag, exact[fine])).all()
+    assert (np.abs(got[fine] - exact[fine]) <= bound(torch, dt, g, a64[fine], wd, exact[fine])).all()
 
 
 def gated_exact(a64, wg, wu, act):
@@ -208,11 +228,9 @@ def test_gated(ctx, torch_cuda, M, K, N, g, zeros, pad, act, dtype):
     dg, du = (dense(q, s, z, g) for q, s, z in mats)
     with np.errstate(over="ignore"):
         gx, ux, f, exact = gated_exact(a64, dg, du, act)
-    e = (4 * LIMBS[dtype] * g / 16 + K / g + 20) * U
-    eg, eu = e * (np.abs(a64) @ np.abs(dg)), e * (np.abs(a64) @ np.abs(du))
-    half = torch.finfo(dt).eps / 2
+    eg, eu = sums_bound(dtype, g, a64, dg), sums_bound(dtype, g, a64, du)
     tol = 1.13 * eg * (np.abs(ux) + eu) + np.abs(f) * eu + 128 * U * np.abs(exact)
-    tol = tol * (1 + half) + half * np.abs(exact) + torch.finfo(dt).smallest_normal * half + 2.0 ** -126
+    tol = rounded(torch, dt, tol, exact) + 2.0 ** -126
     got = h.double().cpu().numpy()
     over = np.abs(exact) > 65000 if dtype == "float16" else np.zeros_like(exact, bool)
     assert (np.abs(got - exact) <= tol)[~over].all(), float((np.abs(got - exact) / tol)[~over].max())
