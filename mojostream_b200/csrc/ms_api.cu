@@ -34,7 +34,6 @@
 #include "ms_pages.h"
 #include "ms_plan.h"
 #include "ms_q4g.h"
-#include "ms_rules.h"
 
 using namespace ms;
 
@@ -370,7 +369,6 @@ extern "C" ms_status ms_init(int device, ms_ctx** out) {
   if (prepare_gemv_stream() != cudaSuccess || prepare_attention() != cudaSuccess ||
       prepare_gemm_tc() != cudaSuccess || prepare_gemm_sk() != cudaSuccess ||
       prepare_lm_tc() != cudaSuccess || prepare_q4g() != cudaSuccess ||
-      prepare_rules() != cudaSuccess ||
       prepare_attention_prefill() != cudaSuccess) {
     ms_destroy(c);
     return MS_ERR_CUDA;

@@ -26,10 +26,8 @@ struct RulesParams {
   long long mask_ld;
   int n_masks;
   const int* mask_row;  // [M], or null: row r uses mask r
-  int chunk;            // columns per CTA, a multiple of 32
 };
 
 cudaError_t launch_rules(const RulesParams& p, int sm_count, cudaStream_t s);
-cudaError_t prepare_rules();
 
 }  // namespace ms

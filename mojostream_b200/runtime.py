@@ -53,12 +53,19 @@ def _stream():
     return ctypes.c_void_p(s if s else _CUDA_STREAM_LEGACY)
 
 
+_raw_stream = None
+
+
 def _stream_on(device):
     """torch's current stream of `device` (see _stream), whichever device is
-    current."""
-    import torch
-    s = torch.cuda.current_stream(device).cuda_stream
-    return s if s else _CUDA_STREAM_LEGACY
+    current, as an int."""
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
+        # the same handle without building a Stream object (1.3 us a call)
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda d: torch.cuda.current_stream(d).cuda_stream)
+    return _raw_stream(device) or _CUDA_STREAM_LEGACY
 
 
 _DTYPES = None

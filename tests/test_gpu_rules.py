@@ -81,6 +81,9 @@ def same(torch, got, want32, dtype):
     (1, 1, 0, 3, 1, 1), (1, 31, 0, 5, 2, 2), (2, 33, 1, 0, 0, 3), (3, 1000, 0, 50, 0, 0),
     (5, 8192, 8, 0, 7, 0), (4, 8193, 0, 300, 5, 4), (37, 32003, 13, 700, 5, 9), (1, 262144, 0, 500, 8, 1),
     (9, 100001, 3, 5000, 60, 5), (2, 4096, 0, 0, 0, 0),
+    # many columns: the stream and the lists in kernels of their own
+    (64, 65536, 0, 300, 9, 7), (40, 70001, 5, 20000, 100, 3), (31, 100003, 1, 40, 0, 0),
+    (70, 50000, 0, 0, 30, 2), (48, 60000, 0, 0, 0, 5),
 ])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_rules(ctx, torch_cuda, M, V, pad, hist, bias, masks, dtype, in_place):
@@ -104,11 +107,11 @@ def test_rules(ctx, torch_cuda, M, V, pad, hist, bias, masks, dtype, in_place):
     same(torch, got, want, dt)
 
 
-def test_each_part_alone_and_masks_by_row(ctx, torch_cuda):
+@pytest.mark.parametrize("M,V", [(6, 3000), (50, 60001)])
+def test_each_part_alone_and_masks_by_row(ctx, torch_cuda, M, V):
     torch = torch_cuda
     rng = np.random.default_rng(4)
-    M, V = 6, 3000
-    x = make(rng, M, V, 100, 6, 6)
+    x = make(rng, M, V, 100, 6, M)
     lg = logits_of(torch, rng, M, V, 0, torch.float32)
     for keep in (("hist", "hist_off"), ("hist", "hist_off", "repetition"),
                  ("hist", "hist_off", "presence"), ("hist", "hist_off", "frequency"),
@@ -116,6 +119,29 @@ def test_each_part_alone_and_masks_by_row(ctx, torch_cuda):
         part = {k: x[k] for k in keep}
         got = ctx.logit_rules(lg, on_gpu(torch, part), out=torch.empty_like(lg))
         same(torch, got, reference(lg.cpu().numpy(), **part), torch.float32)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_more_distinct_ids_than_a_table_holds(ctx, torch_cuda, in_place):
+    """Every id of a large vocabulary in one row's history, some often: each
+    is penalised once, whatever tables the ids pass through."""
+    torch = torch_cuda
+    rng = np.random.default_rng(9)
+    M, V = 20, 150000
+    ids = [np.arange(V), rng.integers(0, V, 30000), np.repeat(rng.integers(0, V, 3), 70000),
+           8 * rng.integers(0, V // 8, 20000), 16384 * rng.integers(0, V // 16384, 500)]
+    ids += [rng.integers(0, V, 50) for _ in range(M - len(ids))]
+    off = np.cumsum([0] + [len(i) for i in ids]).astype(np.int32)
+    x = dict(hist=np.concatenate(ids).astype(np.int32), hist_off=off,
+             repetition=np.full(M, 1.25, np.float32), presence=np.full(M, 0.5, np.float32),
+             frequency=np.full(M, 0.125, np.float32),
+             bias_id=np.tile(np.arange(0, V, 40, dtype=np.int32), M),
+             bias_val=rng.random(M * (V // 40)).astype(np.float32),
+             bias_off=(np.arange(M + 1) * (V // 40)).astype(np.int32))
+    lg = logits_of(torch, rng, M, V, 0, torch.float32)
+    want = reference(lg.cpu().numpy(), **x)
+    got = ctx.logit_rules(lg, on_gpu(torch, x), out=None if in_place else torch.empty_like(lg))
+    same(torch, got, want, torch.float32)
 
 
 def test_offsets_are_clamped(ctx, torch_cuda):
