@@ -369,6 +369,7 @@ extern "C" ms_status ms_init(int device, ms_ctx** out) {
   if (prepare_gemv_stream() != cudaSuccess || prepare_attention() != cudaSuccess ||
       prepare_gemm_tc() != cudaSuccess || prepare_gemm_sk() != cudaSuccess ||
       prepare_lm_tc() != cudaSuccess || prepare_q4g() != cudaSuccess ||
+      prepare_q4g_tc() != cudaSuccess ||
       prepare_attention_prefill() != cudaSuccess) {
     ms_destroy(c);
     return MS_ERR_CUDA;

@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <climits>
+#include <cstdlib>
 #include <cstdio>
 #include <new>
 
@@ -125,6 +126,16 @@ ms_status run_q4g(ms_ctx* c, const ms_q4g_weight* w, const ms_q4g_weight* w2, in
   p.accumulate = accumulate;
   p.act = act;
   p.err = ms_err_word_(c);
+  static const int tcm = getenv("QGTC") ? atoi(getenv("QGTC")) : 9;
+  if (M >= tcm) {
+    if (M > (1 << 22)) OPS_FAIL(c, MS_ERR_SHAPE, "q4g: M=%d", M);
+    void* ws = nullptr;
+    const ms_status st = ms_workspace_(c, s, q4g_planes_bytes(p, ms_sm_count_(c)), &ws);
+    if (st != MS_OK) return st;
+    p.a.records = (uint8_t*)ws;
+    OPS_CUDA(c, launch_q4g_tc(p, ms_sm_count_(c), s));
+    return MS_OK;
+  }
   if ((M + kQgMaxRows - 1) / kQgMaxRows > 65535) OPS_FAIL(c, MS_ERR_SHAPE, "q4g: M=%d", M);
   if (!q4g_stream_converts(p, ms_sm_count_(c))) {
     void* ws = nullptr;

@@ -1,0 +1,104 @@
+// ms_q4g.cuh -- device helpers shared by the kernels of group-scaled 4-bit
+// products (ms_q4g.cu, ms_q4g_tc.cu).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "ms_common.cuh"
+#include "ms_q4g.h"
+
+namespace ms {
+
+__device__ __forceinline__ float u16_scale(uint32_t u, int bf) {
+  return bf ? __uint_as_float(u << 16) : __half2float(__ushort_as_half((unsigned short)u));
+}
+
+// Shared-memory loads by 32-bit address.
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t a) {
+  uint32_t v;
+  asm volatile("{\n .reg .u16 h;\n ld.shared.u16 h, [%1];\n cvt.u32.u16 %0, h;\n}" : "=r"(v) : "r"(a));
+  return v;
+}
+
+// Eight consecutive values of a row (zeros past K, a multiple of 32).
+__device__ __forceinline__ void load8(const Q4gRows& a, int m, int k, float (&v)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = 0.f;
+  if (k >= a.K) return;
+  if (a.type == kQgF32) {
+    const float* x = reinterpret_cast<const float*>(a.a) + (size_t)m * a.lda + k;
+    if (a.vec) {
+      const float4 y = __ldcg(reinterpret_cast<const float4*>(x));
+      const float4 z = __ldcg(reinterpret_cast<const float4*>(x) + 1);
+      v[0] = y.x; v[1] = y.y; v[2] = y.z; v[3] = y.w;
+      v[4] = z.x; v[5] = z.y; v[6] = z.z; v[7] = z.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = __ldcg(x + j);
+    }
+  } else {
+    const unsigned short* x = reinterpret_cast<const unsigned short*>(a.a) + (size_t)m * a.lda + k;
+    uint32_t u[8];
+    if (a.vec) {
+      const uint4 y = __ldcg(reinterpret_cast<const uint4*>(x));
+      const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[j] = (w[j / 2] >> (16 * (j & 1))) & 0xffffu;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[j] = __ldcg(x + j);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      v[j] = a.type == kQgBf16 ? __uint_as_float(u[j] << 16)
+                               : __half2float(__ushort_as_half((unsigned short)u[j]));
+  }
+}
+
+__device__ __forceinline__ float act_fn(float g, int act) {
+  if (act == 0) return g / (1.f + expf(-g));
+  // (1 + tanh u) / 2 = 1 / (1 + e^-2u): no cancellation for negative u
+  const float u = 0.7978845608028654f * (g + 0.044715f * g * g * g);
+  return g / (1.f + expf(-2.f * u));
+}
+
+__device__ __forceinline__ float load_out(const void* p, size_t i, int type) {
+  if (type == kQgF32) return reinterpret_cast<const float*>(p)[i];
+  if (type == kQgBf16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(reinterpret_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ void store_out(void* p, size_t i, int type, float v) {
+  if (type == kQgF32)
+    reinterpret_cast<float*>(p)[i] = v;
+  else if (type == kQgBf16)
+    reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else
+    reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+
+// A finished sum v (gated: gate v, up u) of row m, column n.
+__device__ __forceinline__ void finish(const Q4gParams& p, int m, int n, float v, float u) {
+  if (n >= p.w.N) return;
+  if (p.w2) v = act_fn(v, p.act) * u;
+  const size_t at = (size_t)m * p.ldo + n;
+  if (p.accumulate) v += load_out(p.out, at, p.a.type);
+  store_out(p.out, at, p.a.type, v);
+}
+
+}  // namespace ms

@@ -72,7 +72,7 @@ struct Q4gRows {
   long long lda;
   int type, M, K, nkb, group;
   int vec;           // rows start on 16-byte boundaries
-  uint8_t* records;  // [row block of 8][128-k block]
+  uint8_t* records;  // [row block of 8][128-k block]; many rows: limb planes
 };
 
 struct Q4gParams {
@@ -99,5 +99,10 @@ size_t q4g_records_bytes(const Q4gRows& r);
 bool q4g_stream_converts(const Q4gParams& p, int sm_count);
 cudaError_t launch_q4g_stream(const Q4gParams& p, int sm_count, cudaStream_t s);
 cudaError_t prepare_q4g();
+// Many rows on tcgen05 (ms_q4g_tc.cu): two launches; p.a.records is workspace
+// of q4g_planes_bytes.
+size_t q4g_planes_bytes(const Q4gParams& p, int sm_count);
+cudaError_t launch_q4g_tc(const Q4gParams& p, int sm_count, cudaStream_t s);
+cudaError_t prepare_q4g_tc();
 
 }  // namespace ms
