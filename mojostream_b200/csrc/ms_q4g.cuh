@@ -101,4 +101,45 @@ __device__ __forceinline__ void finish(const Q4gParams& p, int m, int n, float v
   store_out(p.out, at, p.a.type, v);
 }
 
+__device__ __forceinline__ void add4(float4& a, const float4& b) {
+  a.x += b.x;
+  a.y += b.y;
+  a.z += b.z;
+  a.w += b.w;
+}
+
+// finish() of four neighbouring columns, in one store where they are aligned.
+__device__ __forceinline__ void finish4(const Q4gParams& p, int m, int n, const float4& v,
+                                        const float4& u) {
+  const size_t at = (size_t)m * p.ldo + n;
+  const int bytes = p.a.type == kQgF32 ? 16 : 8;
+  uint8_t* d = reinterpret_cast<uint8_t*>(p.out) + at * (bytes / 4);
+  float x[4] = {v.x, v.y, v.z, v.w};
+  if (n + 4 > p.w.N || ((uintptr_t)d & (bytes - 1)) || p.accumulate) {
+    const float y[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll 1
+    for (int e = 0; e < 4; ++e) {
+      const float xe = e == 0 ? x[0] : e == 1 ? x[1] : e == 2 ? x[2] : x[3];
+      const float ye = e == 0 ? y[0] : e == 1 ? y[1] : e == 2 ? y[2] : y[3];
+      finish(p, m, n + e, xe, ye);
+    }
+    return;
+  }
+  if (p.w2) {
+    x[0] = act_fn(x[0], p.act) * u.x;
+    x[1] = act_fn(x[1], p.act) * u.y;
+    x[2] = act_fn(x[2], p.act) * u.z;
+    x[3] = act_fn(x[3], p.act) * u.w;
+  }
+  if (p.a.type == kQgF32) {
+    *reinterpret_cast<float4*>(d) = make_float4(x[0], x[1], x[2], x[3]);
+  } else if (p.a.type == kQgBf16) {
+    __nv_bfloat162 h[2] = {__floats2bfloat162_rn(x[0], x[1]), __floats2bfloat162_rn(x[2], x[3])};
+    *reinterpret_cast<uint2*>(d) = *reinterpret_cast<const uint2*>(h);
+  } else {
+    __half2 h[2] = {__floats2half2_rn(x[0], x[1]), __floats2half2_rn(x[2], x[3])};
+    *reinterpret_cast<uint2*>(d) = *reinterpret_cast<const uint2*>(h);
+  }
+}
+
 }  // namespace ms

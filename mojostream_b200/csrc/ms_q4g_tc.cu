@@ -11,14 +11,18 @@
 // and it is added to fp32 sums in registers.
 //
 // CTA: 128 weight columns on the MMA's M side (gated: 64 of the gate, 64 of
-// the up weight) x NT rows on its N side x a share of the k blocks.  Warp 0
-// streams weight pieces with bulk copies; one thread of warp 1 issues the MMAs; warps 2-9 unpack a 64-k half of the weights into the A
-// operand, then take the groups that the half before completed out of tensor
-// memory (a thread owns one weight column and half of the rows); warp 10
-// streams the limb planes.  Weights,
-// A operand, B operand and accumulators have rings of their own, so unpacking,
-// MMAs and sums of neighbouring halves overlap.  A cluster's CTAs share k; the
-// sums are added in k order through distributed shared memory.
+// the up weight) x NT rows on its N side x a share of the k blocks.  Roles, in
+// warpgroups of four warps that split the register file between them:
+//   0      weight pieces and limb planes by bulk copy; the MMAs
+//   1, 2   unpack the weights of one 64-k half each into the A operand
+//   3, 4   take finished groups out of tensor memory (a thread owns one weight
+//          column and half of the rows)
+// Packed weights, operand stages (HS 64-k halves of A and of every limb of B)
+// and accumulators have rings of their own.  With unpacking and sums on the
+// same eight warps a 128-k block took 2700 cycles against 1024 of MMAs (256
+// rows); with separate rings for A and B the issuing warp's waits took 2200.
+// A cluster's CTAs share k; their sums are added in k order through
+// distributed shared memory.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -31,12 +35,10 @@
 namespace ms {
 namespace {
 
-constexpr int kTqWorkers = 8;
-constexpr int kTqThreads = (3 + kTqWorkers) * kWarp;
+constexpr int kTqThreads = 20 * kWarp;
 constexpr int kTqLboA = 2048 + 32;  // k cores of A: 32 bytes apart in the banks
 constexpr int kTqA = 8 * kTqLboA;   // a 64-k half of 128 columns, bfloat16
-constexpr int kTqStagesA = 3;
-constexpr int kTqMaxB = 12, kTqMaxW = 4, kTqMaxD = 4;
+constexpr int kTqMaxS = 6, kTqMaxW = 4, kTqMaxD = 4;
 constexpr size_t kTqSmemMax = 224 * 1024;
 constexpr int kTqMaxCluster = 8;
 
@@ -89,8 +91,22 @@ __global__ void __launch_bounds__(256) q4g_planes_kernel(const Q4gRows a, int li
 }
 
 // ------------------------------------------------------------- product --
+// Position in a ring of n slots; phase counts the rounds (its parity is the one
+// to wait for).
+struct Ring {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int n, int by = 1) {  // by <= n
+    slot += by;
+    if (slot >= n) {
+      slot -= n;
+      phase ^= 1;
+    }
+  }
+};
+
 struct TcShape {
-  int limbs, nB, nW, nD, cs, row_tiles;
+  int limbs, nS, nW, nD, cs, row_tiles;
 };
 
 // Four bfloat16 pairs of one column: k 0..7 of a core from the words x, y.
@@ -104,51 +120,79 @@ __device__ __forceinline__ uint4 unpack8(uint32_t x, uint32_t y, int shift, uint
   }
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
+// One lane of a converged warp, the same on every call: the compiler then
+// keeps what that lane hands to the tensor core in uniform registers (behind
+// lane == 0 an MMA took 125 cycles to issue).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ void sts128(uint32_t a, const uint4& v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
                : "memory");
 }
 
-// NC: rows per worker thread (the tile has NT = 2 NC); G: 32-k steps per group.
+// Registers a thread of warpgroups 0-2 and of 3-4 holds after the split.  The
+// launch gives every thread `kLaunch` (the register file over 20 warps, or
+// over 40 where two CTAs share an SM); 12 x low + 8 x high <= 20 x kLaunch.
+constexpr __host__ __device__ int halves_per_stage(int NC) { return NC <= 16 ? 2 : 1; }
+template <int NC>
+struct Regs {
+  static constexpr int kCtas = NC <= 32 ? 2 : 1;
+  static constexpr int kLaunch = NC <= 32 ? 48 : 96;
+  static constexpr int kLow = NC <= 32 ? 40 : 48;
+  static constexpr int kHigh = NC <= 16 ? 56 : NC <= 32 ? 56 : 168;
+  static_assert(12 * kLow + 8 * kHigh <= 20 * kLaunch, "register split");
+};
+template <int N>
+__device__ __forceinline__ void reg_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void reg_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// NC: rows per thread that takes sums (the tile has NT = 2 NC); G: 32-k steps
+// per group.
 template <int NC, int G>
-__global__ void __launch_bounds__(kTqThreads, NC <= 32 ? 2 : 1)
+__global__ void __launch_bounds__(kTqThreads, Regs<NC>::kCtas)
     q4g_tc_kernel(const Q4gParams p, const TcShape c) {
-  constexpr int NT = 2 * NC;
+  constexpr int NT = 2 * NC, HS = halves_per_stage(NC);
   extern __shared__ __align__(1024) uint8_t dsm[];
-  __shared__ __align__(8) uint64_t full_w[kTqMaxW], empty_w[kTqMaxW], full_a[kTqStagesA],
-      empty_a[kTqStagesA], full_b[kTqMaxB], empty_b[kTqMaxB], full_d[kTqMaxD], empty_d[kTqMaxD], done;
+  __shared__ __align__(8) uint64_t full_w[kTqMaxW], empty_w[kTqMaxW], full_s[kTqMaxS],
+      empty_s[kTqMaxS], full_d[kTqMaxD], empty_d[kTqMaxD], done;
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_bad;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int nkb = p.w.nkb, bb = p.w.block_bytes;
   const int rank = blockIdx.x % c.cs, tile = blockIdx.x / c.cs, rt = blockIdx.y;
   const int kb0 = nkb * rank / c.cs, kb1 = nkb * (rank + 1) / c.cs;
-  const int steps = (kb1 - kb0) * 2;  // 64-k halves
-  constexpr int kUnitB = NT * 128;    // a limb of a half
+  const int blocks = kb1 - kb0, stages = blocks * 2 / HS;
+  constexpr int kUnitB = NT * 128;  // a limb of a half
   const int stage_w = 2 * kQgQuad * bb;
-  uint8_t* ring_a = dsm;
-  uint8_t* ring_b = ring_a + kTqStagesA * kTqA;
-  uint8_t* ring_w = ring_b + c.nB * kUnitB;
+  // operand stage: HS halves of A, then [HS][limb] units of B
+  const int stage_s = HS * (kTqA + c.limbs * kUnitB);
+  uint8_t* ring_s = dsm;
+  uint8_t* ring_w = dsm + c.nS * stage_s;
   constexpr uint32_t kColsD = NT;
 
   if (threadIdx.x == 0) {
     s_bad = 0;
     for (int s = 0; s < c.nW; ++s) {
       mbar_init(&full_w[s], 1);
-      mbar_init(&empty_w[s], kTqWorkers);
+      mbar_init(&empty_w[s], 8);
     }
-    for (int s = 0; s < kTqStagesA; ++s) {
-      mbar_init(&full_a[s], kTqWorkers);
-      mbar_init(&empty_a[s], 1);
-    }
-    for (int s = 0; s < c.nB; ++s) {
-      mbar_init(&full_b[s], 1);
-      mbar_init(&empty_b[s], 1);
+    for (int s = 0; s < c.nS; ++s) {
+      mbar_init(&full_s[s], 4 * HS + 1);  // the unpacking warps, and the planes' bytes
+      mbar_init(&empty_s[s], 1);
     }
     for (int s = 0; s < c.nD; ++s) {
       mbar_init(&full_d[s], 1);
-      mbar_init(&empty_d[s], kTqWorkers);
+      mbar_init(&empty_d[s], 8);
     }
     mbar_init(&done, 1);
     mbar_fence_init();
@@ -170,246 +214,265 @@ __global__ void __launch_bounds__(kTqThreads, NC <= 32 ? 2 : 1)
     atomicOr(p.err, kErrWaitTimeout);
     s_bad = 1;
   };
+  // the tile's quads of columns (the second may not exist)
+  const size_t quad_bytes = (size_t)nkb * kQgQuad * bb;
+  const uint8_t* w0 = p.w.w + (size_t)tile * (p.w2 ? 1 : 2) * quad_bytes;
+  const uint8_t* w1 = p.w2 ? p.w2 + (size_t)tile * quad_bytes : w0 + quad_bytes;
+  const bool second = p.w2 || tile * 2 + 1 < q4g_quads(p.w.N);
 
-  float acc[NC];
-#pragma unroll
-  for (int i = 0; i < NC; ++i) acc[i] = 0.f;
-  const int wk = warp - 2;              // worker
-  const int quad = warp & 3;            // tensor-memory lanes 32 quad ..
-  const int half_n = wk >> 2;           // rows half_n * NC ..
-  const int col = quad * kWarp + lane;  // the thread's weight column
+  const int row0 = rt * NT, rows = min(NT, p.a.M - row0);
+  constexpr int kLd = 128 + 4;
+  float* S = reinterpret_cast<float*>(dsm);  // [NT][kLd]: staged sums
 
-  if (warp == 0) {
-    // -------------------------------------------------------- producer --
+  if (warp < 4) {
+    reg_dec<Regs<NC>::kLow>();
+    if (warp == 0) {
+    // ------------------------------------------------ weight producer --
     if (lane == 0) {
-      const uint8_t* w0;
-      const uint8_t* w1;  // the tile's two quads (the second may not exist)
-      const size_t quad_bytes = (size_t)nkb * kQgQuad * bb;
-      int second = 1;
-      if (p.w2) {
-        w0 = p.w.w + (size_t)tile * quad_bytes;
-        w1 = p.w2 + (size_t)tile * quad_bytes;
-      } else {
-        w0 = p.w.w + (size_t)tile * 2 * quad_bytes;
-        w1 = w0 + quad_bytes;
-        second = tile * 2 + 1 < q4g_quads(p.w.N);
-      }
-      w0 += (size_t)kb0 * kQgQuad * bb;
-      w1 += (size_t)kb0 * kQgQuad * bb;
-      const int n = kb1 - kb0;
+      const uint8_t* x0 = w0 + (size_t)kb0 * kQgQuad * bb;
+      const uint8_t* x1 = w1 + (size_t)kb0 * kQgQuad * bb;
+      const int n = blocks, run = kQgQuad * bb;
+      Ring w;
       int i = 0;
-      for (; i < n; ++i) {  // no kernel writes the weights: no wait for the previous one
-        const int s = i % c.nW;
-        if (i >= c.nW && !mbar_wait(&empty_w[s], ((i / c.nW) - 1) & 1)) break;
-        uint8_t* st = ring_w + s * stage_w;
-        mbar_expect_tx(&full_w[s], kQgQuad * bb * (1 + second));
-        bulk_g2s(st, w0 + (size_t)i * kQgQuad * bb, kQgQuad * bb, &full_w[s]);
-        if (second) bulk_g2s(st + kQgQuad * bb, w1 + (size_t)i * kQgQuad * bb, kQgQuad * bb, &full_w[s]);
+      for (; i < n; ++i, w.next(c.nW)) {  // no kernel writes the weights: no wait for the previous one
+        if (i >= c.nW && !mbar_wait(&empty_w[w.slot], w.phase ^ 1)) break;
+        uint8_t* st = ring_w + w.slot * stage_w;
+        mbar_expect_tx(&full_w[w.slot], run * (1 + second));
+        bulk_g2s(st, x0, run, &full_w[w.slot]);
+        if (second) bulk_g2s(st + run, x1, run, &full_w[w.slot]);
+        x0 += run;
+        x1 += run;
       }
       if (i < n) fail();
       // the copies issued last land before the CTA can exit
       for (int j = max(0, i - c.nW); j < i; ++j) mbar_wait(&full_w[j % c.nW], (j / c.nW) & 1);
     }
-  } else if (warp == 2 + kTqWorkers) {
+    } else if (warp == 2) {
     // ------------------------------------------------- planes producer --
     if (lane == 0) {
+      const int bytes = HS * c.limbs * kUnitB;
       const uint8_t* b0 = p.a.records + ((size_t)rt * nkb + kb0) * 2 * c.limbs * kUnitB;
-      const int n = steps * c.limbs;
       pdl_wait();
+      Ring u;
       int i = 0;
-      for (; i < n; ++i) {
-        const int s = i % c.nB;
-        if (i >= c.nB && !mbar_wait(&empty_b[s], ((i / c.nB) - 1) & 1)) break;
-        mbar_expect_tx(&full_b[s], kUnitB);
-        bulk_g2s(ring_b + s * kUnitB, b0 + (size_t)i * kUnitB, kUnitB, &full_b[s]);
+      for (; i < stages; ++i, u.next(c.nS)) {
+        if (i >= c.nS && !mbar_wait(&empty_s[u.slot], u.phase ^ 1)) break;
+        mbar_expect_tx(&full_s[u.slot], bytes);
+        bulk_g2s(ring_s + u.slot * stage_s + HS * kTqA, b0, bytes, &full_s[u.slot]);
+        b0 += bytes;
       }
-      if (i < n) fail();
-      for (int j = max(0, i - c.nB); j < i; ++j) mbar_wait(&full_b[j % c.nB], (j / c.nB) & 1);
+      if (i < stages) {
+        fail();
+        // (the copies that were issued: bounded, the unpacking may have stopped)
+        for (int j = max(0, i - c.nS); j < i; ++j) mbar_wait(&full_s[j % c.nS], (j / c.nS) & 1);
+      }
     }
-  } else if (warp == 1) {
+    } else if (warp == 1) {
     // ------------------------------------------------------ MMA issuer --
-    if (lane == 0) {
-      const uint32_t idesc = idesc_bf16(128, NT);
-      const uint32_t a_base = smem_u32(ring_a), b_base = smem_u32(ring_b);
-      int d = -1;  // accumulators used so far - 1
-      for (int j = 0; j < steps; ++j) {
-        const int sa = j % kTqStagesA;
-        bool ok = mbar_wait(&full_a[sa], (j / kTqStagesA) & 1);
-        for (int l = 0; l < c.limbs && ok; ++l) {
-          const int ub = j * c.limbs + l;
-          ok = mbar_wait(&full_b[ub % c.nB], (ub / c.nB) & 1);
-        }
-        // groups inside this half (two of 32, one of 64, or half of one of 128)
-        constexpr int kSub = G == 1 ? 2 : 1, kK16 = 4 / kSub;
-        for (int g = 0; g < kSub && ok; ++g) {
-          const bool begins = G < 4 || (j & 1) == 0;
-          if (begins) {
-            ++d;
-            if (d >= c.nD) ok = mbar_wait(&empty_d[d % c.nD], ((d / c.nD) - 1) & 1);
-            if (!ok) break;
-          }
-          tc_fence_after();
-          const uint32_t dt = tmem + (uint32_t)(d % c.nD) * kColsD;
-          for (int l = 0; l < c.limbs; ++l) {
-            const uint32_t b = b_base + ((j * c.limbs + l) % c.nB) * kUnitB;
-#pragma unroll
-            for (int k = 0; k < kK16; ++k) {
-              const int k16 = g * kK16 + k;
-              umma_bf16(dt, umma_desc(a_base + sa * kTqA + 2 * k16 * kTqLboA, kTqLboA, 128),
-                        umma_desc(b + 2 * k16 * NT * 16, NT * 16, 128), idesc,
-                        !(begins && l == 0 && k == 0));
-            }
-          }
-          if (G < 4 || (j & 1)) umma_commit(&full_d[d % c.nD]);
-        }
-        if (!ok) {
-          fail();
-          break;
-        }
-        umma_commit(&empty_a[sa]);
-        for (int l = 0; l < c.limbs; ++l) umma_commit(&empty_b[(j * c.limbs + l) % c.nB]);
-      }
-      umma_commit(&done);  // arrives when every MMA issued above has finished
-    }
-  } else {
-    // --------------------------------------- unpacking and group sums --
-    const int r = lane >> 2, t = lane & 3;
-    const uint32_t ring_a_s = smem_u32(ring_a), ring_w_s = smem_u32(ring_w);
-    constexpr int ng = 4 / G, kSub = G == 1 ? 2 : 1;
-    const bool live = p.w2 || wk < 4 || tile * 2 + 1 < q4g_quads(p.w.N);  // the tile's quad exists
-    float sc[kSub] = {};  // scales of the groups of the half before
-    int d = 0;
-    // the group sums of accumulator d, scaled
-    auto take = [&](float s) -> bool {
-      const int sd = d % c.nD;
-      if (!mbar_wait(&full_d[sd], (d / c.nD) & 1)) return false;
-      tc_fence_after();
-      const uint32_t ta = tmem + ((uint32_t)(quad * kWarp) << 16) + (uint32_t)(sd * (int)kColsD + half_n * NC);
-#pragma unroll
-      for (int i = 0; i < NC; i += 16) {
-        uint32_t v[16];
-        tmem_ld16(ta + i, v);
-        tmem_wait_ld();
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i + e] = fmaf(s, __uint_as_float(v[e]), acc[i + e]);
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty_d[sd]);
-      ++d;
-      return true;
-    };
+    // (the whole warp walks the loop, one lane issues)
+    const uint32_t idesc = idesc_bf16(128, NT);
+    const uint64_t desc_a = umma_desc(smem_u32(ring_s), kTqLboA, 128);
+    const uint64_t desc_b = umma_desc(smem_u32(ring_s) + HS * kTqA, NT * 16, 128);
+    constexpr uint32_t kStepA = 2 * kTqLboA / 16, kStepB = 2 * NT;  // 16 k, in 16-byte units
+    // groups that a half completes (32: two, 64: one, 128: every second half one)
+    constexpr int kSub = G == 1 ? 2 : 1, kK16 = 4 / kSub;
+    Ring rs, rd;
+    int used = 0;  // accumulators begun
     bool ok = true;
-    for (int j = 0; j < steps && ok; ++j) {
-      const int kb = j >> 1, half = j & 1, sw = kb % c.nW, sa = j % kTqStagesA;
-      ok = mbar_wait(&full_w[sw], (kb / c.nW) & 1) &&
-           (j < kTqStagesA || mbar_wait(&empty_a[sa], ((j / kTqStagesA) - 1) & 1));
-      if (!ok) break;
-      const uint32_t st = ring_w_s + sw * stage_w;
-      // warp wk unpacks tile wk of the 128 columns
-      const uint32_t pc = st + wk * bb;
-      const uint32_t dst = ring_a_s + sa * kTqA + t * kTqLboA + wk * 256 + r * 16;
-      if (live) {
-        const uint4 w = lds128(pc + half * 512 + lane * 16);
-        uint32_t lo[2], hi[2];  // biases of the half's two 32-k steps
+    auto wait = [&](uint64_t* bar, uint32_t phase) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, phase)) != 0;
+    };
+    for (int j = 0; j < stages && ok; ++j, rs.next(c.nS)) {
+      ok = wait(&full_s[rs.slot], rs.phase);
+      const uint64_t da = desc_a + (uint32_t)(rs.slot * stage_s / 16);
+      const uint64_t db = desc_b + (uint32_t)(rs.slot * stage_s / 16);
+      tc_fence_after();
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          lo[hh] = hi[hh] = 0x43084308u;  // 128 + 8
-          if (p.w.zeros) {
-            const uint32_t z = lds16(pc + kQgNibbles + ng * 32 + ((2 * half + hh) / G * 8 + r) * 2);
-            lo[hh] = (0x4300u | (z & 0xffu)) * 0x10001u;
-            hi[hh] = (0x4300u | (z >> 8)) * 0x10001u;
+      for (int h = 0; h < HS; ++h) {
+        const bool odd = HS == 2 ? h == 1 : (j & 1) != 0;
+#pragma unroll
+        for (int g = 0; g < kSub; ++g) {
+          const bool begins = G < 4 || !odd, ends = G < 4 || odd;
+          if (begins) {
+            if (used >= c.nD) {
+              ok = ok && wait(&empty_d[rd.slot], rd.phase ^ 1);
+              tc_fence_after();
+            }
+            ++used;
           }
-        }
-        sts128(dst, unpack8(w.x, w.y, 0, lo[0]));
-        sts128(dst + 128, unpack8(w.x, w.y, 4, hi[0]));
-        sts128(dst + 4 * kTqLboA, unpack8(w.z, w.w, 0, lo[1]));
-        sts128(dst + 4 * kTqLboA + 128, unpack8(w.z, w.w, 4, hi[1]));
-      }
-      // scales of this half's groups for the thread's column
-      float sn[kSub];
+          const uint32_t dt = tmem + (uint32_t)rd.slot * kColsD;
+          if (ok && elect_one()) {
+            for (int l = 0; l < c.limbs; ++l) {
+              const uint64_t dbl = db + (uint32_t)((h * c.limbs + l) * (kUnitB / 16));
 #pragma unroll
-      for (int g = 0; g < kSub; ++g) {
-        const int grp = G == 1 ? 2 * half + g : half * 2 / G;
-        const uint32_t at = st + (col >> 4) * bb + kQgNibbles + ((grp * 8 + (col & 7)) * 2 + ((col >> 3) & 1)) * 2;
-        sn[g] = u16_scale(lds16(at), p.w.bf_scale);
+              for (int k = 0; k < kK16; ++k)
+                umma_bf16(dt, da + h * (kTqA / 16) + (g * kK16 + k) * kStepA, dbl + (g * kK16 + k) * kStepB,
+                          idesc, k != 0 || l != 0 || !begins);
+            }
+            if (ends) umma_commit(&full_d[rd.slot]);
+            if (h == HS - 1 && g == kSub - 1) umma_commit(&empty_s[rs.slot]);
+          }
+          if (ends) rd.next(c.nD);
+        }
+      }
+    }
+    if (!ok && lane == 0) fail();
+    if (elect_one()) umma_commit(&done);  // arrives when every MMA issued above has finished
+    __syncwarp();
+    }
+  } else if (warp < 12) {
+    // ----------------------------------------------------- unpacking --
+    // warps 4-7 the first half of each block, 8-11 the second; two tiles each
+    reg_dec<Regs<NC>::kLow>();
+    const int half = (warp - 4) >> 2, i = warp & 3;
+    const int r = lane >> 2, t = lane & 3;
+    const uint32_t ring_a = smem_u32(ring_s), ring_w_s = smem_u32(ring_w);
+    constexpr int ng = 4 / G;
+    const bool live = second || i < 2;  // the tiles exist
+    Ring rs, rw;
+    if (HS == 1) rs.next(c.nS, half);
+    for (int kb = 0; kb < blocks; ++kb) {
+      if (!mbar_wait(&full_w[rw.slot], rw.phase)) {
+        if (lane == 0) fail();
+        break;
+      }
+      const uint32_t pc = ring_w_s + rw.slot * stage_w + 2 * i * bb;
+      const uint4 x[2] = {lds128(pc + half * 512 + lane * 16), lds128(pc + bb + half * 512 + lane * 16)};
+      uint32_t z[2][2] = {{0x0808u, 0x0808u}, {0x0808u, 0x0808u}};
+      if (p.w.zeros)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh)
+            z[j][hh] = lds16(pc + j * bb + kQgNibbles + ng * 32 + ((2 * half + hh) / G * 8 + r) * 2);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty_w[rw.slot]);
+      rw.next(c.nW);
+      if ((HS == 1 ? 2 * kb + half : kb) >= c.nS && !mbar_wait(&empty_s[rs.slot], rs.phase ^ 1)) {
+        if (lane == 0) fail();
+        break;
+      }
+      if (live) {
+        const uint32_t dst = ring_a + rs.slot * stage_s + (HS == 2 ? half * kTqA : 0) + t * kTqLboA +
+                             2 * i * 256 + r * 16;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t l0 = (0x4300u | (z[j][0] & 0xffu)) * 0x10001u, h0 = (0x4300u | (z[j][0] >> 8)) * 0x10001u;
+          const uint32_t l1 = (0x4300u | (z[j][1] & 0xffu)) * 0x10001u, h1 = (0x4300u | (z[j][1] >> 8)) * 0x10001u;
+          sts128(dst + j * 256, unpack8(x[j].x, x[j].y, 0, l0));
+          sts128(dst + j * 256 + 128, unpack8(x[j].x, x[j].y, 4, h0));
+          sts128(dst + j * 256 + 4 * kTqLboA, unpack8(x[j].z, x[j].w, 0, l1));
+          sts128(dst + j * 256 + 4 * kTqLboA + 128, unpack8(x[j].z, x[j].w, 4, h1));
+        }
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&full_a[sa]);
-        if (half) mbar_arrive(&empty_w[sw]);
-      }
-      if (j > 0) {
-#pragma unroll
-        for (int g = 0; g < kSub; ++g)
-          if (ok && (G < 4 || half == 0)) ok = take(sc[g]);
-      }
-#pragma unroll
-      for (int g = 0; g < kSub; ++g) sc[g] = sn[g];
+      if (lane == 0) mbar_arrive(&full_s[rs.slot]);
+      rs.next(c.nS, HS == 1 ? 2 : 1);
     }
+  } else {
+    // ----------------------------------------------------- group sums --
+    reg_inc<Regs<NC>::kHigh>();
+    const int quad = warp & 3;                  // tensor-memory lanes 32 quad ..
+    const int half_n = (warp - 12) >> 2;        // rows half_n * NC ..
+    const int col = quad * kWarp + lane;        // the thread's weight column
+    float2 acc[NC / 2];
 #pragma unroll
-    for (int g = 0; g < kSub; ++g)
-      if (ok) ok = take(sc[g]);
+    for (int i = 0; i < NC / 2; ++i) acc[i] = make_float2(0.f, 0.f);
+    // the column's scales, a block ahead, from the weight's pieces (in L2)
+    constexpr int ng = 4 / G;
+    const bool exists = second || quad < 2;
+    const uint8_t* scales = (quad < 2 ? w0 : w1) + (size_t)kb0 * kQgQuad * bb + ((col & 63) >> 4) * bb +
+                            kQgNibbles + ((col & 7) * 2 + ((col >> 3) & 1)) * 2;
+    unsigned short sn[ng];
+    auto fetch = [&]() {
+#pragma unroll
+      for (int g = 0; g < ng; ++g)
+        sn[g] = exists ? __ldg(reinterpret_cast<const unsigned short*>(scales + g * 32)) : 0;
+      scales += kQgQuad * bb;
+    };
+    fetch();
+    Ring rd;
+    bool ok = true;
+    for (int kb = 0; kb < blocks && ok; ++kb) {
+      float sc[ng];
+#pragma unroll
+      for (int g = 0; g < ng; ++g) sc[g] = u16_scale(sn[g], p.w.bf_scale);
+      if (kb + 1 < blocks) fetch();
+#pragma unroll
+      for (int g = 0; g < ng; ++g) {
+        ok = ok && mbar_wait(&full_d[rd.slot], rd.phase);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t ta = tmem + ((uint32_t)(quad * kWarp) << 16) + (uint32_t)(rd.slot * (int)kColsD + half_n * NC);
+        const float2 s2 = make_float2(sc[g], sc[g]);
+#pragma unroll
+        for (int i = 0; i < NC; i += 16) {
+          uint32_t v[16];
+          tmem_ld16(ta + i, v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            fma2(acc[i / 2 + e], make_float2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), s2);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty_d[rd.slot]);
+        rd.next(c.nD);
+      }
+    }
     if (!ok && lane == 0) fail();
     if (!mbar_wait(&done, 0) && lane == 0) fail();  // no MMA is in flight
+    tc_fence_before();
+    __syncthreads();
+    // --------------------------------------------------------- results --
+    // by way of shared memory (every copy into it has landed: the MMAs and the
+    // unpacking waited for them), rows of 128 columns, four to a thread
+    int bad = s_bad;
+    pdl_wait();  // results may overwrite what the previous kernel still reads
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      S[(half_n * NC + i) * kLd + col] = i & 1 ? acc[i / 2].y : acc[i / 2].x;
+    if (c.cs > 1) {
+      cluster_arrive();
+      cluster_wait();
+      const uint32_t bad0 = smem_u32(const_cast<int*>(&s_bad));
+      for (int k = 0; k < c.cs; ++k) bad |= ld_dsmem_s32(dsmem_addr(bad0, (uint32_t)k));
+    } else {
+      bar_sync_n(1, 8 * kWarp);
+    }
+    if (!bad) {  // no results after a wait that ran out
+      const int out_cols = p.w2 ? 64 : 128, sh = p.w2 ? 4 : 5;
+      // the rows of this rank: m = rank, rank + cs, ...
+      const int mine = rank < rows ? (rows - rank + c.cs - 1) / c.cs : 0;
+      for (int i = threadIdx.x - 12 * kWarp; i < mine << sh; i += 8 * kWarp) {
+        const int m = rank + (i >> sh) * c.cs, n0 = 4 * (i & ((1 << sh) - 1));
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f), u = v;
+        const float* at = S + m * kLd + n0;
+        if (c.cs > 1) {
+          for (int k = 0; k < c.cs; ++k) add4(v, ld_dsmem4(dsmem_addr(smem_u32(at), (uint32_t)k)));
+          if (p.w2)
+            for (int k = 0; k < c.cs; ++k) add4(u, ld_dsmem4(dsmem_addr(smem_u32(at + 64), (uint32_t)k)));
+        } else {
+          v = *reinterpret_cast<const float4*>(at);
+          if (p.w2) u = *reinterpret_cast<const float4*>(at + 64);
+        }
+        finish4(p, row0 + m, tile * out_cols + n0, v, u);
+      }
+    }
+    if (c.cs > 1) {  // the other CTAs have read this one's sums
+      cluster_arrive();
+      cluster_wait();
+    }
+    return;
   }
-
-  // ------------------------------------------------------------- results --
-  // rows m of this tile, the thread's column: straight to memory (32 columns
-  // of a row per warp), or, gated and in a cluster, by way of shared memory
-  tc_fence_before();
+  // warps 0-11 (few registers): the takers' barriers, and the tensor memory back
   __syncthreads();
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem, cols);
-  const int row0 = rt * NT, rows = min(NT, p.a.M - row0);
-  int bad = s_bad;
-  constexpr int kLd = 128 + 4;
-  float* S = reinterpret_cast<float*>(dsm);  // [NT][kLd]
-  const bool staged = p.w2 || c.cs > 1;
-  if (wk >= 0 && wk < kTqWorkers) {
-    pdl_wait();  // results may overwrite what the previous kernel still reads
-    if (!staged) {
-      const int n = tile * 128 + col;
-      if (!bad && n < p.w.N) {
-#pragma unroll
-        for (int i = 0; i < NC; ++i)
-          if (half_n * NC + i < rows) finish(p, row0 + half_n * NC + i, n, acc[i], 0.f);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NC; ++i) S[(half_n * NC + i) * kLd + col] = acc[i];
-    }
-  }
-  if (!staged) return;
-  __syncthreads();
   if (c.cs > 1) {
     cluster_arrive();
     cluster_wait();
-    const uint32_t bad0 = smem_u32(const_cast<int*>(&s_bad));
-    for (int k = 0; k < c.cs; ++k) bad |= ld_dsmem_s32(dsmem_addr(bad0, (uint32_t)k));
-  }
-  if (!bad) {
-    pdl_wait();
-    const int out_cols = p.w2 ? 64 : 128, sh = p.w2 ? 6 : 7;
-    // the rows of this rank: m = rank, rank + cs, ...
-    const int mine = rank < rows ? (rows - rank + c.cs - 1) / c.cs : 0;
-    for (int i = threadIdx.x; i < mine << sh; i += kTqThreads) {
-      const int m = rank + (i >> sh) * c.cs, n0 = i & (out_cols - 1);
-      float v = 0.f, u = 0.f;
-      if (c.cs > 1) {
-        const uint32_t at = smem_u32(S + m * kLd + n0);
-        for (int k = 0; k < c.cs; ++k) v += ld_dsmem(dsmem_addr(at, (uint32_t)k));
-        if (p.w2)
-          for (int k = 0; k < c.cs; ++k) u += ld_dsmem(dsmem_addr(at + 256, (uint32_t)k));
-      } else {
-        v = S[m * kLd + n0];
-        u = S[m * kLd + n0 + 64];
-      }
-      finish(p, row0 + m, tile * out_cols + n0, v, u);
-    }
-  }
-  if (c.cs > 1) {  // the other CTAs have read this one's sums
     cluster_arrive();
     cluster_wait();
   }
@@ -442,21 +505,22 @@ TcPlan plan_tc(const Q4gParams& p, int sm_count) {
          p.w.nkb >= 4 * o.c.cs)
     o.c.cs *= 2;
   o.c.nD = o.NC <= 64 ? 4 : 2;
-  const size_t limit = o.NC <= 32 ? 112 * 1024 : kTqSmemMax;
+  const size_t limit = o.NC <= 32 ? kTqSmemMax / 2 : kTqSmemMax;
   const size_t stage_w = 2 * (size_t)kQgQuad * p.w.block_bytes, unit = (size_t)o.NC * 256;
+  const int hs = halves_per_stage(o.NC);
+  const size_t stage_s = hs * (kTqA + o.c.limbs * unit);
+  o.c.nS = 2;
   o.c.nW = 2;
-  o.c.nB = 2 * o.c.limbs;
-  size_t smem = kTqStagesA * kTqA + o.c.nW * stage_w + o.c.nB * unit;
-  // what is left: more stages of the weights, then of the planes
+  size_t smem = o.c.nS * stage_s + o.c.nW * stage_w;
+  while (o.c.nS < kTqMaxS && smem + stage_s <= limit) {
+    ++o.c.nS;
+    smem += stage_s;
+  }
   while (o.c.nW < kTqMaxW && smem + stage_w <= limit) {
     ++o.c.nW;
     smem += stage_w;
   }
-  while (o.c.nB + o.c.limbs <= kTqMaxB && smem + o.c.limbs * unit <= limit) {
-    o.c.nB += o.c.limbs;
-    smem += o.c.limbs * unit;
-  }
-  const size_t staged = p.w2 || o.c.cs > 1 ? (size_t)2 * o.NC * 132 * 4 : 0;
+  const size_t staged = (size_t)2 * o.NC * 132 * 4;
   o.smem = staged > smem ? staged : smem;
   return o;
 }
