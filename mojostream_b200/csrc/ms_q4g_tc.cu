@@ -14,9 +14,10 @@
 // the up weight) x NT rows on its N side x a share of the k blocks.  Roles, in
 // warpgroups of four warps that split the register file between them:
 //   0      weight pieces and limb planes by bulk copy; the MMAs
-//   1, 2   unpack the weights of one 64-k half each into the A operand
-//   3, 4   take finished groups out of tensor memory (a thread owns one weight
-//          column and half of the rows)
+//   1-2    unpack the weights into the A operand (1-4 for 32-row tiles, where
+//          the weights' stream is the bound)
+//   last 2 take finished groups out of tensor memory: a thread owns one weight
+//          column and half of the rows (one warpgroup and all rows for 32)
 // Packed weights, operand stages (HS 64-k halves of A and of every limb of B)
 // and accumulators have rings of their own.  With unpacking and sums on the
 // same eight warps a 128-k block took 2700 cycles against 1024 of MMAs (256
@@ -35,7 +36,6 @@
 namespace ms {
 namespace {
 
-constexpr int kTqThreads = 20 * kWarp;
 constexpr int kTqLboA = 2048 + 32;  // k cores of A: 32 bytes apart in the banks
 constexpr int kTqA = 8 * kTqLboA;   // a 64-k half of 128 columns, bfloat16
 constexpr int kTqMaxS = 6, kTqMaxW = 4, kTqMaxD = 4;
@@ -134,17 +134,23 @@ __device__ __forceinline__ void sts128(uint32_t a, const uint4& v) {
                : "memory");
 }
 
-// Registers a thread of warpgroups 0-2 and of 3-4 holds after the split.  The
-// launch gives every thread `kLaunch` (the register file over 20 warps, or
-// over 40 where two CTAs share an SM); 12 x low + 8 x high <= 20 x kLaunch.
-constexpr __host__ __device__ int halves_per_stage(int NC) { return NC <= 16 ? 2 : 1; }
-template <int NC>
-struct Regs {
-  static constexpr int kCtas = NC <= 32 ? 2 : 1;
-  static constexpr int kLaunch = NC <= 32 ? 48 : 96;
-  static constexpr int kLow = NC <= 32 ? 40 : 48;
-  static constexpr int kHigh = NC <= 16 ? 56 : NC <= 32 ? 56 : 168;
-  static_assert(12 * kLow + 8 * kHigh <= 20 * kLaunch, "register split");
+// Shape of a kernel for tiles of NT rows.  Registers: the launch gives every
+// thread kLaunch; then warpgroup 0 and the unpacking ones keep kLow, those
+// that hold sums take kHigh.
+template <int NT>
+struct Tile {
+  static constexpr int kCtas = NT <= 64 ? 2 : 1;    // CTAs per SM
+  static constexpr int HS = NT <= 32 ? 2 : 1;       // 64-k halves of an operand stage
+  static constexpr int kUnpackWg = NT <= 32 ? 4 : 2, kTakeWg = NT <= 32 ? 1 : 2;
+  static constexpr int kWg = 1 + kUnpackWg + kTakeWg;
+  static constexpr int kThreads = kWg * 4 * kWarp;
+  static constexpr int kTakeWarp0 = 4 * (1 + kUnpackWg);
+  static constexpr int TC = NT / kTakeWg;           // rows per thread that holds sums
+  static constexpr int kLaunch = NT <= 32 ? 40 : NT <= 64 ? 48 : 96;
+  static constexpr int kLow = NT <= 32 ? 32 : NT <= 64 ? 40 : 48;
+  static constexpr int kHigh = NT <= 32 ? 80 : NT <= 64 ? 56 : 168;
+  static_assert((1 + kUnpackWg) * kLow + kTakeWg * kHigh <= kWg * kLaunch, "register split");
+  static_assert(kCtas * kThreads * kLaunch <= 65536, "register file");
 };
 template <int N>
 __device__ __forceinline__ void reg_dec() {
@@ -155,12 +161,12 @@ __device__ __forceinline__ void reg_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-// NC: rows per thread that takes sums (the tile has NT = 2 NC); G: 32-k steps
-// per group.
-template <int NC, int G>
-__global__ void __launch_bounds__(kTqThreads, Regs<NC>::kCtas)
+// NT: rows of the tile; G: 32-k steps per group.
+template <int NT, int G>
+__global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
     q4g_tc_kernel(const Q4gParams p, const TcShape c) {
-  constexpr int NT = 2 * NC, HS = halves_per_stage(NC);
+  using S_ = Tile<NT>;
+  constexpr int HS = S_::HS;
   extern __shared__ __align__(1024) uint8_t dsm[];
   __shared__ __align__(8) uint64_t full_w[kTqMaxW], empty_w[kTqMaxW], full_s[kTqMaxS],
       empty_s[kTqMaxS], full_d[kTqMaxD], empty_d[kTqMaxD], done;
@@ -184,15 +190,15 @@ __global__ void __launch_bounds__(kTqThreads, Regs<NC>::kCtas)
     s_bad = 0;
     for (int s = 0; s < c.nW; ++s) {
       mbar_init(&full_w[s], 1);
-      mbar_init(&empty_w[s], 8);
+      mbar_init(&empty_w[s], 4 * S_::kUnpackWg);
     }
     for (int s = 0; s < c.nS; ++s) {
-      mbar_init(&full_s[s], 4 * HS + 1);  // the unpacking warps, and the planes' bytes
+      mbar_init(&full_s[s], 2 * HS * S_::kUnpackWg + 1);  // the unpacking warps, and the planes' bytes
       mbar_init(&empty_s[s], 1);
     }
     for (int s = 0; s < c.nD; ++s) {
       mbar_init(&full_d[s], 1);
-      mbar_init(&empty_d[s], 8);
+      mbar_init(&empty_d[s], 4 * S_::kTakeWg);
     }
     mbar_init(&done, 1);
     mbar_fence_init();
@@ -225,7 +231,7 @@ __global__ void __launch_bounds__(kTqThreads, Regs<NC>::kCtas)
   float* S = reinterpret_cast<float*>(dsm);  // [NT][kLd]: staged sums
 
   if (warp < 4) {
-    reg_dec<Regs<NC>::kLow>();
+    reg_dec<S_::kLow>();
     if (warp == 0) {
     // ------------------------------------------------ weight producer --
     if (lane == 0) {
@@ -276,16 +282,29 @@ __global__ void __launch_bounds__(kTqThreads, Regs<NC>::kCtas)
     constexpr uint32_t kStepA = 2 * kTqLboA / 16, kStepB = 2 * NT;  // 16 k, in 16-byte units
     // groups that a half completes (32: two, 64: one, 128: every second half one)
     constexpr int kSub = G == 1 ? 2 : 1, kK16 = 4 / kSub;
+    // a wait costs this warp as much as two MMAs, so those of the next stage are
+    // taken while half of this one's MMAs are still to issue; with an accumulator
+    // to wait for in every half that would hold MMAs back for the sums' warps
+    // (groups of 32, 2048 rows: 222 us, and 255 us so), so only for groups of 128
+    constexpr bool kAhead = G == 4;
     Ring rs, rd;
     int used = 0;  // accumulators begun
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t phase) {
       return __all_sync(0xffffffffu, mbar_wait(bar, phase)) != 0;
     };
-    for (int j = 0; j < stages && ok; ++j, rs.next(c.nS)) {
-      ok = wait(&full_s[rs.slot], rs.phase);
+    // stage rs, and the accumulator rd if its first group begins one there
+    auto ready = [&](bool begins) {
+      return wait(&full_s[rs.slot], rs.phase) &&
+             (!begins || used < c.nD || wait(&empty_d[rd.slot], rd.phase ^ 1));
+    };
+    if (kAhead) ok = ready(true);
+    for (int j = 0; j < stages && ok; ++j) {
+      if (!kAhead) ok = wait(&full_s[rs.slot], rs.phase);
       const uint64_t da = desc_a + (uint32_t)(rs.slot * stage_s / 16);
       const uint64_t db = desc_b + (uint32_t)(rs.slot * stage_s / 16);
+      const int slot = rs.slot;
+      rs.next(c.nS);
       tc_fence_after();
 #pragma unroll
       for (int h = 0; h < HS; ++h) {
@@ -293,26 +312,42 @@ __global__ void __launch_bounds__(kTqThreads, Regs<NC>::kCtas)
 #pragma unroll
         for (int g = 0; g < kSub; ++g) {
           const bool begins = G < 4 || !odd, ends = G < 4 || odd;
+          const bool last = h == HS - 1 && g == kSub - 1;
           if (begins) {
-            if (used >= c.nD) {
+            if (!kAhead && used >= c.nD) {
               ok = ok && wait(&empty_d[rd.slot], rd.phase ^ 1);
               tc_fence_after();
             }
             ++used;
           }
           const uint32_t dt = tmem + (uint32_t)rd.slot * kColsD;
+          auto issue = [&](int l, int k) {
+            umma_bf16(dt, da + h * (kTqA / 16) + (g * kK16 + k) * kStepA,
+                      db + (uint32_t)((h * c.limbs + l) * (kUnitB / 16)) + (g * kK16 + k) * kStepB, idesc,
+                      k != 0 || l != 0 || !begins);
+          };
+          constexpr int kNow = kAhead ? kK16 / 2 : kK16;  // of a stage's last limb before the waits
           if (ok && elect_one()) {
-            for (int l = 0; l < c.limbs; ++l) {
-              const uint64_t dbl = db + (uint32_t)((h * c.limbs + l) * (kUnitB / 16));
+            for (int l = 0; l + 1 < c.limbs; ++l)
 #pragma unroll
-              for (int k = 0; k < kK16; ++k)
-                umma_bf16(dt, da + h * (kTqA / 16) + (g * kK16 + k) * kStepA, dbl + (g * kK16 + k) * kStepB,
-                          idesc, k != 0 || l != 0 || !begins);
-            }
-            if (ends) umma_commit(&full_d[rd.slot]);
-            if (h == HS - 1 && g == kSub - 1) umma_commit(&empty_s[rs.slot]);
+              for (int k = 0; k < kK16; ++k) issue(l, k);
+#pragma unroll
+            for (int k = 0; k < (last ? kNow : kK16); ++k) issue(c.limbs - 1, k);
+            if ((!last || !kAhead) && ends) umma_commit(&full_d[rd.slot]);
+            if (last && !kAhead) umma_commit(&empty_s[slot]);
           }
+          const int sd = rd.slot;
           if (ends) rd.next(c.nD);
+          if (kAhead && last) {
+            const bool more = j + 1 >= stages || ready(HS == 2 || odd);
+            if (ok && elect_one()) {
+#pragma unroll
+              for (int k = kNow; k < kK16; ++k) issue(c.limbs - 1, k);
+              if (ends) umma_commit(&full_d[sd]);
+              umma_commit(&empty_s[slot]);
+            }
+            ok = ok && more;
+          }
         }
       }
     }
@@ -320,15 +355,17 @@ __global__ void __launch_bounds__(kTqThreads, Regs<NC>::kCtas)
     if (elect_one()) umma_commit(&done);  // arrives when every MMA issued above has finished
     __syncwarp();
     }
-  } else if (warp < 12) {
+  } else if (warp < S_::kTakeWarp0) {
     // ----------------------------------------------------- unpacking --
-    // warps 4-7 the first half of each block, 8-11 the second; two tiles each
-    reg_dec<Regs<NC>::kLow>();
-    const int half = (warp - 4) >> 2, i = warp & 3;
+    // half of the warps the first half of each block, the others the second;
+    // kTiles neighbouring tiles to a warp
+    reg_dec<S_::kLow>();
+    constexpr int kTiles = 4 / S_::kUnpackWg;
+    const int half = (warp - 4) / (2 * S_::kUnpackWg), tile0 = (warp - 4) % (2 * S_::kUnpackWg) * kTiles;
     const int r = lane >> 2, t = lane & 3;
     const uint32_t ring_a = smem_u32(ring_s), ring_w_s = smem_u32(ring_w);
     constexpr int ng = 4 / G;
-    const bool live = second || i < 2;  // the tiles exist
+    const bool live = second || tile0 < 4;  // the tiles exist
     Ring rs, rw;
     if (HS == 1) rs.next(c.nS, half);
     for (int kb = 0; kb < blocks; ++kb) {
@@ -336,15 +373,18 @@ __global__ void __launch_bounds__(kTqThreads, Regs<NC>::kCtas)
         if (lane == 0) fail();
         break;
       }
-      const uint32_t pc = ring_w_s + rw.slot * stage_w + 2 * i * bb;
-      const uint4 x[2] = {lds128(pc + half * 512 + lane * 16), lds128(pc + bb + half * 512 + lane * 16)};
-      uint32_t z[2][2] = {{0x0808u, 0x0808u}, {0x0808u, 0x0808u}};
-      if (p.w.zeros)
+      const uint32_t pc = ring_w_s + rw.slot * stage_w + tile0 * bb;
+      uint4 x[kTiles];
+      uint32_t z[kTiles][2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < kTiles; ++j) {
+        x[j] = lds128(pc + j * bb + half * 512 + lane * 16);
+        z[j][0] = z[j][1] = 0x0808u;
+        if (p.w.zeros)
 #pragma unroll
           for (int hh = 0; hh < 2; ++hh)
             z[j][hh] = lds16(pc + j * bb + kQgNibbles + ng * 32 + ((2 * half + hh) / G * 8 + r) * 2);
+      }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty_w[rw.slot]);
       rw.next(c.nW);
@@ -354,9 +394,9 @@ __global__ void __launch_bounds__(kTqThreads, Regs<NC>::kCtas)
       }
       if (live) {
         const uint32_t dst = ring_a + rs.slot * stage_s + (HS == 2 ? half * kTqA : 0) + t * kTqLboA +
-                             2 * i * 256 + r * 16;
+                             tile0 * 256 + r * 16;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < kTiles; ++j) {
           const uint32_t l0 = (0x4300u | (z[j][0] & 0xffu)) * 0x10001u, h0 = (0x4300u | (z[j][0] >> 8)) * 0x10001u;
           const uint32_t l1 = (0x4300u | (z[j][1] & 0xffu)) * 0x10001u, h1 = (0x4300u | (z[j][1] >> 8)) * 0x10001u;
           sts128(dst + j * 256, unpack8(x[j].x, x[j].y, 0, l0));
@@ -372,13 +412,14 @@ __global__ void __launch_bounds__(kTqThreads, Regs<NC>::kCtas)
     }
   } else {
     // ----------------------------------------------------- group sums --
-    reg_inc<Regs<NC>::kHigh>();
+    reg_inc<S_::kHigh>();
+    constexpr int TC = S_::TC;
     const int quad = warp & 3;                  // tensor-memory lanes 32 quad ..
-    const int half_n = (warp - 12) >> 2;        // rows half_n * NC ..
+    const int part = (warp - S_::kTakeWarp0) >> 2;  // rows part * TC ..
     const int col = quad * kWarp + lane;        // the thread's weight column
-    float2 acc[NC / 2];
+    float2 acc[TC / 2];
 #pragma unroll
-    for (int i = 0; i < NC / 2; ++i) acc[i] = make_float2(0.f, 0.f);
+    for (int i = 0; i < TC / 2; ++i) acc[i] = make_float2(0.f, 0.f);
     // the column's scales, a block ahead, from the weight's pieces (in L2)
     constexpr int ng = 4 / G;
     const bool exists = second || quad < 2;
@@ -404,10 +445,10 @@ __global__ void __launch_bounds__(kTqThreads, Regs<NC>::kCtas)
         ok = ok && mbar_wait(&full_d[rd.slot], rd.phase);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t ta = tmem + ((uint32_t)(quad * kWarp) << 16) + (uint32_t)(rd.slot * (int)kColsD + half_n * NC);
+        const uint32_t ta = tmem + ((uint32_t)(quad * kWarp) << 16) + (uint32_t)(rd.slot * (int)kColsD + part * TC);
         const float2 s2 = make_float2(sc[g], sc[g]);
 #pragma unroll
-        for (int i = 0; i < NC; i += 16) {
+        for (int i = 0; i < TC; i += 16) {
           uint32_t v[16];
           tmem_ld16(ta + i, v);
           tmem_wait_ld();
@@ -431,22 +472,24 @@ __global__ void __launch_bounds__(kTqThreads, Regs<NC>::kCtas)
     int bad = s_bad;
     pdl_wait();  // results may overwrite what the previous kernel still reads
 #pragma unroll
-    for (int i = 0; i < NC; ++i)
-      S[(half_n * NC + i) * kLd + col] = i & 1 ? acc[i / 2].y : acc[i / 2].x;
+    for (int i = 0; i < TC; ++i)
+      S[(part * TC + i) * kLd + col] = i & 1 ? acc[i / 2].y : acc[i / 2].x;
     if (c.cs > 1) {
       cluster_arrive();
       cluster_wait();
       const uint32_t bad0 = smem_u32(const_cast<int*>(&s_bad));
       for (int k = 0; k < c.cs; ++k) bad |= ld_dsmem_s32(dsmem_addr(bad0, (uint32_t)k));
     } else {
-      bar_sync_n(1, 8 * kWarp);
+      bar_sync_n(1, 4 * S_::kTakeWg * kWarp);
     }
     if (!bad) {  // no results after a wait that ran out
       const int out_cols = p.w2 ? 64 : 128, sh = p.w2 ? 4 : 5;
-      // the rows of this rank: m = rank, rank + cs, ...
-      const int mine = rank < rows ? (rows - rank + c.cs - 1) / c.cs : 0;
-      for (int i = threadIdx.x - 12 * kWarp; i < mine << sh; i += 8 * kWarp) {
-        const int m = rank + (i >> sh) * c.cs, n0 = 4 * (i & ((1 << sh) - 1));
+      // the rows of this rank, m = rank, rank + cs, ..., four columns to a thread
+      constexpr int kTakers = S_::kTakeWg * 4 * kWarp;
+      const int i0 = threadIdx.x - S_::kTakeWarp0 * kWarp, n0 = 4 * (i0 & ((1 << sh) - 1));
+      const int step = (kTakers >> sh) * c.cs;
+#pragma unroll 2
+      for (int m = rank + (i0 >> sh) * c.cs; m < rows; m += step) {
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f), u = v;
         const float* at = S + m * kLd + n0;
         if (c.cs > 1) {
@@ -466,7 +509,7 @@ __global__ void __launch_bounds__(kTqThreads, Regs<NC>::kCtas)
     }
     return;
   }
-  // warps 0-11 (few registers): the takers' barriers, and the tensor memory back
+  // the other warps (few registers): the takers' barriers, and the tensor memory back
   __syncthreads();
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem, cols);
@@ -479,12 +522,20 @@ __global__ void __launch_bounds__(kTqThreads, Regs<NC>::kCtas)
 }
 
 struct TcPlan {
-  int NC, tiles;
+  int NT, tiles;
   TcShape c;
   size_t smem;
 };
 
 int tc_limbs(int type) { return type == kQgF32 ? 3 : type == kQgF16 ? 2 : 1; }
+
+// Clusters of cs CTAs that run at the same time, with `ctas` CTAs to an SM:
+// asked of the driver once (prepare_q4g_tc), or an even spread.
+int g_clusters[3][kTqMaxCluster + 1];  // [CTAs per SM][cs]
+long long clusters_at_once(int sm_count, int ctas, int cs) {
+  const int n = g_clusters[ctas][cs];
+  return n > 0 ? n : (long long)ctas * sm_count / cs;
+}
 
 TcPlan plan_tc(const Q4gParams& p, int sm_count) {
   TcPlan o{};
@@ -492,26 +543,22 @@ TcPlan plan_tc(const Q4gParams& p, int sm_count) {
   // rows per tile: as few tiles as fit (256 rows of one limb, 128 of more),
   // all of about the same size
   const int most = o.c.limbs == 1 ? 256 : 128;
-  const int tiles = (p.a.M + most - 1) / most, each = (p.a.M + tiles - 1) / tiles;
-  const int widths[5] = {16, 32, 64, 96, 128};
-  o.NC = 128;
+  const int row_tiles = (p.a.M + most - 1) / most, each = (p.a.M + row_tiles - 1) / row_tiles;
+  const int sizes[5] = {32, 64, 128, 192, 256};
+  o.NT = 256;
   for (int i = 4; i >= 0; --i)
-    if (each <= 2 * widths[i]) o.NC = widths[i];
-  o.c.row_tiles = (p.a.M + 2 * o.NC - 1) / (2 * o.NC);
+    if (each <= sizes[i]) o.NT = sizes[i];
+  o.c.row_tiles = (p.a.M + o.NT - 1) / o.NT;
   o.tiles = p.w2 ? q4g_quads(p.w.N) : (q4g_quads(p.w.N) + 1) / 2;
-  // k shared by a cluster while the CTAs do not fill the GPU
-  o.c.cs = 1;
-  while (o.c.cs < kTqMaxCluster && (long long)o.tiles * o.c.row_tiles * o.c.cs * 2 <= sm_count * 5 / 4 &&
-         p.w.nkb >= 4 * o.c.cs)
-    o.c.cs *= 2;
-  o.c.nD = o.NC <= 64 ? 4 : 2;
-  const size_t limit = o.NC <= 32 ? kTqSmemMax / 2 : kTqSmemMax;
-  const size_t stage_w = 2 * (size_t)kQgQuad * p.w.block_bytes, unit = (size_t)o.NC * 256;
-  const int hs = halves_per_stage(o.NC);
-  const size_t stage_s = hs * (kTqA + o.c.limbs * unit);
+  // operand stages: at least two; what is left goes to them, then to the weights
+  const size_t limit = o.NT <= 64 ? kTqSmemMax / 2 : kTqSmemMax;
+  const size_t stage_w = 2 * (size_t)kQgQuad * p.w.block_bytes;
+  const size_t stage_s = (o.NT <= 32 ? 2 : 1) * (kTqA + (size_t)o.c.limbs * o.NT * 128);
   o.c.nS = 2;
   o.c.nW = 2;
+  o.c.nD = o.NT <= 128 ? 4 : 2;
   size_t smem = o.c.nS * stage_s + o.c.nW * stage_w;
+  const int ctas = smem <= limit && o.NT <= 64 ? 2 : 1;  // per SM
   while (o.c.nS < kTqMaxS && smem + stage_s <= limit) {
     ++o.c.nS;
     smem += stage_s;
@@ -520,17 +567,31 @@ TcPlan plan_tc(const Q4gParams& p, int sm_count) {
     ++o.c.nW;
     smem += stage_w;
   }
-  const size_t staged = (size_t)2 * o.NC * 132 * 4;
+  const size_t staged = (size_t)o.NT * 132 * 4;
   o.smem = staged > smem ? staged : smem;
+  // k shared by the CTAs of a cluster: the split with the least rounds x (blocks
+  // of a CTA + what a CTA costs besides, about ten blocks).  A cluster's CTAs
+  // share a GPC, so what fits at once is counted in clusters (16 rows, K 13824,
+  // N 5120: 40 clusters of seven do not, 39 us; of six they do, 29 us).
+  const long long grid = (long long)o.tiles * o.c.row_tiles;
+  long long best = 0;
+  for (int cs = 1; cs <= kTqMaxCluster && (cs == 1 || p.w.nkb >= 4 * cs); ++cs) {
+    const long long slots = clusters_at_once(sm_count, ctas, cs);
+    const long long cost = (grid + slots - 1) / slots * ((p.w.nkb + cs - 1) / cs + 10);
+    if (cs == 1 || cost < best) {
+      best = cost;
+      o.c.cs = cs;
+    }
+  }
   return o;
 }
 
-template <int NC, int G>
+template <int NT, int G>
 cudaError_t launch_tc_t(const Q4gParams& p, const TcPlan& o, cudaStream_t s) {
   if (o.smem > kTqSmemMax) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(o.tiles * o.c.cs, o.c.row_tiles, 1);
-  cfg.blockDim = dim3(kTqThreads);
+  cfg.blockDim = dim3(Tile<NT>::kThreads);
   cfg.dynamicSmemBytes = o.smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
@@ -545,28 +606,51 @@ cudaError_t launch_tc_t(const Q4gParams& p, const TcPlan& o, cudaStream_t s) {
     attr[1].val.clusterDim.z = 1;
     cfg.numAttrs = 2;
   }
-  return cudaLaunchKernelEx(&cfg, q4g_tc_kernel<NC, G>, p, o.c);
+  return cudaLaunchKernelEx(&cfg, q4g_tc_kernel<NT, G>, p, o.c);
 }
 
-template <int NC>
+template <int NT>
 cudaError_t launch_tc_g(const Q4gParams& p, const TcPlan& o, cudaStream_t s) {
   switch (p.w.group) {
-    case 32: return launch_tc_t<NC, 1>(p, o, s);
-    case 64: return launch_tc_t<NC, 2>(p, o, s);
-    default: return launch_tc_t<NC, 4>(p, o, s);
+    case 32: return launch_tc_t<NT, 1>(p, o, s);
+    case 64: return launch_tc_t<NT, 2>(p, o, s);
+    default: return launch_tc_t<NT, 4>(p, o, s);
   }
 }
 
-template <int NC, int G>
+template <int NT>
+void count_clusters(int ctas) {
+  for (int cs = kTqMaxCluster; cs >= 1; --cs) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(cs * 1024);
+    cfg.blockDim = dim3(Tile<NT>::kThreads);
+    cfg.dynamicSmemBytes = kTqSmemMax / ctas;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)cs;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, q4g_tc_kernel<NT, 4>, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      n = 0;
+    }
+    g_clusters[ctas][cs] = n;
+  }
+}
+
+template <int NT, int G>
 cudaError_t prepare_tc_t() {
-  return cudaFuncSetAttribute(q4g_tc_kernel<NC, G>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  return cudaFuncSetAttribute(q4g_tc_kernel<NT, G>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                               (int)kTqSmemMax);
 }
-template <int NC>
+template <int NT>
 cudaError_t prepare_tc_g() {
-  cudaError_t e = prepare_tc_t<NC, 1>();
-  if (e == cudaSuccess) e = prepare_tc_t<NC, 2>();
-  if (e == cudaSuccess) e = prepare_tc_t<NC, 4>();
+  cudaError_t e = prepare_tc_t<NT, 1>();
+  if (e == cudaSuccess) e = prepare_tc_t<NT, 2>();
+  if (e == cudaSuccess) e = prepare_tc_t<NT, 4>();
   return e;
 }
 
@@ -574,7 +658,7 @@ cudaError_t prepare_tc_g() {
 
 size_t q4g_planes_bytes(const Q4gParams& p, int sm_count) {
   const TcPlan o = plan_tc(p, sm_count);
-  return (size_t)o.c.row_tiles * 2 * o.NC * p.w.nkb * kQgBlockK * 2 * o.c.limbs;
+  return (size_t)o.c.row_tiles * o.NT * p.w.nkb * kQgBlockK * 2 * o.c.limbs;
 }
 
 cudaError_t launch_q4g_tc(const Q4gParams& p, int sm_count, cudaStream_t s) {
@@ -589,24 +673,28 @@ cudaError_t launch_q4g_tc(const Q4gParams& p, int sm_count, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, q4g_planes_kernel, p.a, o.c.limbs, 2 * o.NC);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, q4g_planes_kernel, p.a, o.c.limbs, o.NT);
   if (e != cudaSuccess) return e;
-  switch (o.NC) {
-    case 16: return launch_tc_g<16>(p, o, s);
+  switch (o.NT) {
     case 32: return launch_tc_g<32>(p, o, s);
     case 64: return launch_tc_g<64>(p, o, s);
-    case 96: return launch_tc_g<96>(p, o, s);
     case 128: return launch_tc_g<128>(p, o, s);
+    case 192: return launch_tc_g<192>(p, o, s);
+    case 256: return launch_tc_g<256>(p, o, s);
   }
   return cudaErrorInvalidValue;
 }
 
 cudaError_t prepare_q4g_tc() {
-  cudaError_t e = prepare_tc_g<16>();
-  if (e == cudaSuccess) e = prepare_tc_g<32>();
+  cudaError_t e = prepare_tc_g<32>();
   if (e == cudaSuccess) e = prepare_tc_g<64>();
-  if (e == cudaSuccess) e = prepare_tc_g<96>();
   if (e == cudaSuccess) e = prepare_tc_g<128>();
+  if (e == cudaSuccess) e = prepare_tc_g<192>();
+  if (e == cudaSuccess) e = prepare_tc_g<256>();
+  if (e == cudaSuccess && !g_clusters[1][1]) {  // (every GPU of a node is alike)
+    count_clusters<64>(2);
+    count_clusters<256>(1);
+  }
   return e;
 }
 
