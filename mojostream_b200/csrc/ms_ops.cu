@@ -4,7 +4,6 @@
 #include <cuda_runtime.h>
 
 #include <climits>
-#include <cstdlib>
 #include <cstdio>
 #include <new>
 
@@ -126,8 +125,7 @@ ms_status run_q4g(ms_ctx* c, const ms_q4g_weight* w, const ms_q4g_weight* w2, in
   p.accumulate = accumulate;
   p.act = act;
   p.err = ms_err_word_(c);
-  static const int tcm = getenv("QGTC") ? atoi(getenv("QGTC")) : 9;
-  if (M >= tcm) {
+  if (M >= q4g_tc_rows(dtype)) {
     if (M > (1 << 22)) OPS_FAIL(c, MS_ERR_SHAPE, "q4g: M=%d", M);
     void* ws = nullptr;
     const ms_status st = ms_workspace_(c, s, q4g_planes_bytes(p, ms_sm_count_(c)), &ws);

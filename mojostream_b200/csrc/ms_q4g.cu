@@ -407,8 +407,12 @@ __global__ void __launch_bounds__(kQgWarps* kWarp, T* NB <= 2 ? 2 : 1)
         }
       }
     }
-    __syncwarp();  // every lane has read the stage
-    if (lane == 0 && i + p.stages < n) {
+    // Every lane's loads from the stage have arrived before it is refilled: the
+    // last of them is in this sum, and a sum is never this NaN (a barrier alone
+    // does not wait for loads in flight)
+    const unsigned read = __ballot_sync(
+        0xffffffffu, __float_as_uint(acc[T - 1][NB - 1][1]) != 0x7fedcba9u);
+    if (lane == 0 && read && i + p.stages < n) {
       issue_w(slot);
       if (!own_a) issue_a(slot, i_kb);
       advance();

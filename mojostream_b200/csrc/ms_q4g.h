@@ -101,6 +101,10 @@ cudaError_t launch_q4g_stream(const Q4gParams& p, int sm_count, cudaStream_t s);
 cudaError_t prepare_q4g();
 // Many rows on tcgen05 (ms_q4g_tc.cu): two launches; p.a.records is workspace
 // of q4g_planes_bytes.
+// From how many rows on: 9 bfloat16 rows (K 13824, N 5120: 32 us, two rounds of
+// the streaming kernel 37 us; at 24 rows 33 and 50 us), 17 rows that take two or
+// three limbs (K 5120, N 13824 fp32: 16 rows 48 and 36 us, 32 rows 48 and 66 us).
+inline int q4g_tc_rows(int type) { return type == kQgBf16 ? 9 : 17; }
 size_t q4g_planes_bytes(const Q4gParams& p, int sm_count);
 cudaError_t launch_q4g_tc(const Q4gParams& p, int sm_count, cudaStream_t s);
 cudaError_t prepare_q4g_tc();

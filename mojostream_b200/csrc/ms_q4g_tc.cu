@@ -385,9 +385,6 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
           for (int hh = 0; hh < 2; ++hh)
             z[j][hh] = lds16(pc + j * bb + kQgNibbles + ng * 32 + ((2 * half + hh) / G * 8 + r) * 2);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty_w[rw.slot]);
-      rw.next(c.nW);
       if ((HS == 1 ? 2 * kb + half : kb) >= c.nS && !mbar_wait(&empty_s[rs.slot], rs.phase ^ 1)) {
         if (lane == 0) fail();
         break;
@@ -407,7 +404,14 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&full_s[rs.slot]);
+      if (lane == 0) {
+        mbar_arrive(&full_s[rs.slot]);
+        // only now: what was unpacked depends on the loads from this slot, which
+        // the arrival would not have waited for (the MMAs' reads of shared memory
+        // can hold loads up until the next copy has landed)
+        mbar_arrive(&empty_w[rw.slot]);
+      }
+      rw.next(c.nW);
       rs.next(c.nS, HS == 1 ? 2 : 1);
     }
   } else {
@@ -546,7 +550,9 @@ TcPlan plan_tc(const Q4gParams& p, int sm_count) {
   const int row_tiles = (p.a.M + most - 1) / most, each = (p.a.M + row_tiles - 1) / row_tiles;
   const int sizes[5] = {32, 64, 128, 192, 256};
   o.NT = 256;
-  for (int i = 4; i >= 0; --i)
+  // (with limbs a 32-row tile's stages leave one CTA to an SM: 24 rows fp32, K
+  // 2560, N 20480 took 62 us so and 50 us in tiles of 64)
+  for (int i = 4; i >= (o.c.limbs > 1 ? 1 : 0); --i)
     if (each <= sizes[i]) o.NT = sizes[i];
   o.c.row_tiles = (p.a.M + o.NT - 1) / o.NT;
   o.tiles = p.w2 ? q4g_quads(p.w.N) : (q4g_quads(p.w.N) + 1) / 2;
