@@ -502,11 +502,12 @@ StreamPlan plan_stream(const Q4gParams& p, int sm_count) {
   const int quads = q4g_quads(p.w.N) * (p.w2 ? 2 : 1);
   o.T = o.NB <= 2 && quads >= sm_count ? 4 : 2;
   o.sets = quads * kQgQuad / o.T;
-  // rows x blocks that 16 warps convert in three rounds (about 1 us); more
-  // come converted (2 us, mostly the launch, at any size)
+  // rows x blocks that 16 warps convert in two rounds (one or two rows: three);
+  // more come converted, a launch more (one row, K 10240, N 5120 fp32: 14.4 us,
+  // and 17.3 us; four rows, K 2560: 8.1 and 7.3 us)
   const size_t rec = (size_t)qg_record_bytes(rows, p.w.group);
   const size_t a_all = p.w.nkb * rec;
-  o.a_smem = row_blocks == 1 && rows * p.w.nkb <= 6 * kQgWarps && a_all <= 64 * 1024 ? a_all : 0;
+  o.a_smem = row_blocks == 1 && rows * p.w.nkb <= (rows <= 2 ? 6 : 4) * kQgWarps && a_all <= 64 * 1024 ? a_all : 0;
   const size_t stage = (size_t)o.T * p.w.block_bytes + (o.a_smem ? 0 : rec);
   const size_t fixed = o.a_smem + (size_t)kQgWarps * 2 * rows * o.T * kQgTile * sizeof(float);
   // small sets run two CTAs to an SM (64 registers)
