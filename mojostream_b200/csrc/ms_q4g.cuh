@@ -71,11 +71,19 @@ __device__ __forceinline__ void load8(const Q4gRows& a, int m, int k, float (&v)
   }
 }
 
-__device__ __forceinline__ float act_fn(float g, int act) {
-  if (act == 0) return g / (1.f + expf(-g));
-  // (1 + tanh u) / 2 = 1 / (1 + e^-2u): no cancellation for negative u
-  const float u = 0.7978845608028654f * (g + 0.044715f * g * g * g);
-  return g / (1.f + expf(-2.f * u));
+// SiLU: g / (1 + e^-g); GELU: (1 + tanh u) / 2 = 1 / (1 + e^-2u), without
+// cancellation for negative u.
+__device__ __forceinline__ float act_arg(float g, int act) {
+  return act == 0 ? g : 2.f * 0.7978845608028654f * (g + 0.044715f * g * g * g);
+}
+__device__ __forceinline__ float act_wide(float g, int act) { return g / (1.f + expf(-act_arg(g, act))); }
+// For results of 16 bits: the approximate exponential (of a rounded argument x:
+// |x| 2^-24 relative, 2^-17 before the result vanishes) and reciprocal (2^-23).
+__device__ __forceinline__ float act_narrow(float g, int act) {
+  float e, r;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * act_arg(g, act)));
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return g * r;
 }
 
 __device__ __forceinline__ float load_out(const void* p, size_t i, int type) {
@@ -95,7 +103,7 @@ __device__ __forceinline__ void store_out(void* p, size_t i, int type, float v) 
 // A finished sum v (gated: gate v, up u) of row m, column n.
 __device__ __forceinline__ void finish(const Q4gParams& p, int m, int n, float v, float u) {
   if (n >= p.w.N) return;
-  if (p.w2) v = act_fn(v, p.act) * u;
+  if (p.w2) v = (p.a.type == kQgF32 ? act_wide(v, p.act) : act_narrow(v, p.act)) * u;
   const size_t at = (size_t)m * p.ldo + n;
   if (p.accumulate) v += load_out(p.out, at, p.a.type);
   store_out(p.out, at, p.a.type, v);
@@ -126,10 +134,23 @@ __device__ __forceinline__ void finish4(const Q4gParams& p, int m, int n, const 
     return;
   }
   if (p.w2) {
-    x[0] = act_fn(x[0], p.act) * u.x;
-    x[1] = act_fn(x[1], p.act) * u.y;
-    x[2] = act_fn(x[2], p.act) * u.z;
-    x[3] = act_fn(x[3], p.act) * u.w;
+    if (p.a.type == kQgF32) {
+#pragma unroll 1  // (its code is long: the loop turns the four through one place)
+      for (int e = 0; e < 4; ++e) {
+        const float y = act_wide(x[0], p.act);
+        x[0] = x[1];
+        x[1] = x[2];
+        x[2] = x[3];
+        x[3] = y;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = act_narrow(x[e], p.act);
+    }
+    x[0] *= u.x;
+    x[1] *= u.y;
+    x[2] *= u.z;
+    x[3] *= u.w;
   }
   if (p.a.type == kQgF32) {
     *reinterpret_cast<float4*>(d) = make_float4(x[0], x[1], x[2], x[3]);
@@ -140,6 +161,29 @@ __device__ __forceinline__ void finish4(const Q4gParams& p, int m, int n, const 
     __half2 h[2] = {__floats2half2_rn(x[0], x[1]), __floats2half2_rn(x[2], x[3])};
     *reinterpret_cast<uint2*>(d) = *reinterpret_cast<const uint2*>(h);
   }
+}
+
+// Eight columns of a product that is only rounded and stored, 16-byte aligned.
+__device__ __forceinline__ void store8(const Q4gParams& p, int m, int n, const float4& a,
+                                       const float4& b) {
+  const size_t at = (size_t)m * p.ldo + n;
+  if (p.a.type == kQgF32) {
+    float4* d = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at);
+    d[0] = a;
+    d[1] = b;
+    return;
+  }
+  uint4 o;
+  if (p.a.type == kQgBf16) {
+    const __nv_bfloat162 h[4] = {__floats2bfloat162_rn(a.x, a.y), __floats2bfloat162_rn(a.z, a.w),
+                                 __floats2bfloat162_rn(b.x, b.y), __floats2bfloat162_rn(b.z, b.w)};
+    o = *reinterpret_cast<const uint4*>(h);
+  } else {
+    const __half2 h[4] = {__floats2half2_rn(a.x, a.y), __floats2half2_rn(a.z, a.w),
+                          __floats2half2_rn(b.x, b.y), __floats2half2_rn(b.z, b.w)};
+    o = *reinterpret_cast<const uint4*>(h);
+  }
+  *reinterpret_cast<uint4*>(reinterpret_cast<unsigned short*>(p.out) + at) = o;
 }
 
 }  // namespace ms

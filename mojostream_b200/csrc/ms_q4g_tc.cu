@@ -10,20 +10,28 @@
 // of one group of k over all limbs; when the group ends its scale is applied
 // and it is added to fp32 sums in registers.
 //
-// CTA: 128 weight columns on the MMA's M side (gated: 64 of the gate, 64 of
-// the up weight) x NT rows on its N side x a share of the k blocks.  Roles, in
-// warpgroups of four warps that split the register file between them:
+// CTA: tiles of 128 weight columns on the MMA's M side (gated: 64 of the gate,
+// 64 of the up weight, in turns of 16) x NT rows on its N side x a share of the
+// k blocks.  Roles, in warpgroups of four warps that split the register file
+// between them:
 //   0      weight pieces and limb planes by bulk copy; the MMAs
 //   1-2    unpack the weights into the A operand (1-4 for 32-row tiles, where
 //          the weights' stream is the bound)
 //   last 2 take finished groups out of tensor memory: a thread owns one weight
 //          column and half of the rows (one warpgroup and all rows for 32)
-// Packed weights, operand stages (HS 64-k halves of A and of every limb of B)
-// and accumulators have rings of their own.  With unpacking and sums on the
-// same eight warps a 128-k block took 2700 cycles against 1024 of MMAs (256
-// rows); with separate rings for A and B the issuing warp's waits took 2200.
-// A cluster's CTAs share k; their sums are added in k order through
+// The A operand lies in tensor memory, written in the weights' fragment order:
+// in shared memory its 64 KB of traffic a block and the MMA's own reads were
+// the bound (an MMA of 32 rows took 40 cycles so, and takes 17).  That leaves
+// 384 of 512 columns for accumulators: tiles of at most 192 rows.
+// The roles walk the CTA's tiles without a break, so weights and planes of the
+// next tile are there when it begins.  Where there are too few tiles, a
+// cluster's CTAs share the k of one; their sums are added in k order through
 // distributed shared memory.
+// Every role's loop shares the SM's instruction cache with the others, and its
+// length is what bounds them: with unrolled limbs and the next stage's waits
+// among the MMAs 2048 rows (K 2560, N 10240, bfloat16) took 137 us, and take
+// 103 us (1045 TFLOP/s; 4096 x 5120 x 13824 593 us, 978 TFLOP/s), with the
+// activation's exact division unrolled 519 gated rows took 114 us, and take 98.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -36,57 +44,55 @@
 namespace ms {
 namespace {
 
-constexpr int kTqLboA = 2048 + 32;  // k cores of A: 32 bytes apart in the banks
-constexpr int kTqA = 8 * kTqLboA;   // a 64-k half of 128 columns, bfloat16
-constexpr int kTqMaxS = 6, kTqMaxW = 4, kTqMaxD = 4;
-constexpr size_t kTqSmemMax = 224 * 1024;
+constexpr int kTqMaxS = 4, kTqMaxW = 8, kTqMaxD = 3;
+// dynamic shared memory of a CTA, alone on its SM or one of two
+constexpr size_t kTqSmemMax = 224 * 1024, kTqSmemHalf = 110 * 1024;
 constexpr int kTqMaxCluster = 8;
+constexpr int kChunk = 32;  // rows of a chunk of results
 
 // -------------------------------------------------------------- planes --
-// v = hi + mid + lo exactly: each limb is the leading 8 bits of what is left
-// (truncated, so nothing can round up to infinity).  An infinity or a NaN
-// stays in the first limb alone.
-__device__ __forceinline__ void limbs3(float v, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
-  const uint32_t u = __float_as_uint(v);
-  hi = u & 0xffff0000u;
-  float r = v - __uint_as_float(hi);
+// The next limb of v, the leading 8 bits of what is left (truncated, so nothing
+// can round up to infinity).  An infinity or a NaN stays in the first limb alone.
+__device__ __forceinline__ uint32_t next_limb(float& v) {
+  const uint32_t u = __float_as_uint(v), top = u & 0xffff0000u;
   if ((u & 0x7f800000u) == 0x7f800000u) {
-    if (u & 0x007fffffu) hi |= 0x00400000u;  // a NaN whose payload sits in the low bits
-    r = 0.f;
+    v = 0.f;
+    return u & 0x007fffffu ? top | 0x00400000u : top;  // a NaN's payload may sit in the low bits
   }
-  mid = __float_as_uint(r) & 0xffff0000u;
-  lo = __float_as_uint(r - __uint_as_float(mid));  // at most 8 bits: exact
+  v -= __uint_as_float(top);
+  return top;
 }
 
-// Planes [row tile][64-k half][limb][8 k cores][NT rows][16 bytes]: the B
-// operand's core matrices.  Thread: 8 k (a core) of one row; rows past M are
-// left as they are (their columns of the product are not used).
-__global__ void __launch_bounds__(256) q4g_planes_kernel(const Q4gRows a, int limbs, int NT) {
+// Planes [row tile][64-k half][limb][NT rows][128 bytes, swizzled]: the B
+// operand.  The weights' fragments put k 8 t + 2 j and the one after it, of each
+// 32 k, into column 4 j + t of the A operand, so the 16-byte piece j of the 32 k
+// holds those pairs for t = 0..3.  Thread: 32 k of one row; rows past M
+// are left as they are (their columns of the product are not used).
+__global__ void __launch_bounds__(128) q4g_planes_kernel(const Q4gRows a, int limbs, int NT) {
   pdl_wait();     // the rows are an earlier kernel's output, and the planes
   pdl_trigger();  // may still be read by the product before this one
-  // eight neighbouring threads: the eight rows of a core matrix; then k
-  const int cores = a.nkb * 16;
+  // eight neighbouring threads: eight rows; then k
+  const int spans = a.nkb * 4;
   for (int m8 = blockIdx.y; m8 < (a.M + 7) / 8; m8 += gridDim.y) {
-    const int m = m8 * 8 + (threadIdx.x & 7), core = blockIdx.x * 32 + (threadIdx.x >> 3);
-    if (m >= a.M || core >= cores) continue;
-    float v[8];
-    load8(a, m, core * 8, v);
-    uint32_t l[3][8];
+    const int m = m8 * 8 + (threadIdx.x & 7), span = blockIdx.x * 16 + (threadIdx.x >> 3);
+    if (m >= a.M || span >= spans) continue;
+    float v[4][8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (limbs == 1)
-        l[0][j] = __float_as_uint(v[j]);
-      else
-        limbs3(v[j], l[0][j], l[1][j], l[2][j]);
-    }
+    for (int t = 0; t < 4; ++t) load8(a, m, span * 32 + t * 8, v[t]);
     const int rt = m / NT, r = m % NT;
-    uint8_t* dst = a.records + (((size_t)rt * a.nkb * 2 + (core >> 3)) * limbs * 8 + (core & 7)) * NT * 16 + r * 16;
+    uint8_t* dst = a.records +
+                   (((size_t)rt * a.nkb * 2 + (span >> 1)) * limbs * NT + r) * 128;
+    for (int l = 0; l < limbs; ++l, dst += NT * 128)
 #pragma unroll
-    for (int i = 0; i < 3; ++i)
-      if (i < limbs)
-        *reinterpret_cast<uint4*>(dst + (size_t)i * 8 * NT * 16) = make_uint4(
-            __byte_perm(l[i][0], l[i][1], 0x7632), __byte_perm(l[i][2], l[i][3], 0x7632),
-            __byte_perm(l[i][4], l[i][5], 0x7632), __byte_perm(l[i][6], l[i][7], 0x7632));
+      for (int j = 0; j < 4; ++j) {
+        uint32_t w[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const uint32_t lo = next_limb(v[t][2 * j]), hi = next_limb(v[t][2 * j + 1]);
+          w[t] = __byte_perm(lo, hi, 0x7632);
+        }
+        *reinterpret_cast<uint4*>(dst + ((((span & 1) * 4 + j) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
   }
 }
 
@@ -106,19 +112,18 @@ struct Ring {
 };
 
 struct TcShape {
-  int limbs, nS, nW, nD, cs, row_tiles;
+  int limbs, nS, nW, cs, row_tiles;
+  int tiles, units;  // column tiles; tiles in all
 };
 
-// Four bfloat16 pairs of one column: k 0..7 of a core from the words x, y.
-__device__ __forceinline__ uint4 unpack8(uint32_t x, uint32_t y, int shift, uint32_t bias) {
-  uint32_t o[4];
+// Four bfloat16 pairs of one column, k 0..7 of the words x, y, into every other of r.
+__device__ __forceinline__ void unpack8(uint32_t x, uint32_t y, int shift, uint32_t bias, uint32_t* r) {
   const uint32_t w[4] = {x >> shift, x >> (8 + shift), y >> shift, y >> (8 + shift)};
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const uint32_t v = (w[e] & 0x000F000Fu) | 0x43004300u;
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(o[e]) : "r"(v), "r"(bias));
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r[2 * e]) : "r"(v), "r"(bias));
   }
-  return make_uint4(o[0], o[1], o[2], o[3]);
 }
 // One lane of a converged warp, the same on every call: the compiler then
 // keeps what that lane hands to the tensor core in uniform registers (behind
@@ -129,10 +134,6 @@ __device__ __forceinline__ bool elect_one() {
       "{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}" : "=r"(p));
   return p != 0;
 }
-__device__ __forceinline__ void sts128(uint32_t a, const uint4& v) {
-  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-               : "memory");
-}
 
 // Shape of a kernel for tiles of NT rows.  Registers: the launch gives every
 // thread kLaunch; then warpgroup 0 and the unpacking ones keep kLow, those
@@ -140,10 +141,16 @@ __device__ __forceinline__ void sts128(uint32_t a, const uint4& v) {
 template <int NT>
 struct Tile {
   static constexpr int kCtas = NT <= 64 ? 2 : 1;    // CTAs per SM
-  static constexpr int HS = NT <= 32 ? 2 : 1;       // 64-k halves of an operand stage
+  static constexpr int HS = NT == 32 || NT == 192 ? 2 : 1;       // 64-k halves of an operand stage
   static constexpr int kUnpackWg = NT <= 32 ? 4 : 2, kTakeWg = NT <= 32 ? 1 : 2;
   static constexpr int kWg = 1 + kUnpackWg + kTakeWg;
   static constexpr int kThreads = kWg * 4 * kWarp;
+  // tensor memory: accumulators, then operand stages of 32 columns to a half
+  static constexpr int kCols = 512 / kCtas;
+  static constexpr int kD = NT == 128 ? 3 : 2;
+  static constexpr int kMaxS = (kCols - kD * NT) / (32 * HS);
+  static_assert(kD <= kTqMaxD && kMaxS >= 2, "tensor memory");
+  static constexpr bool kWalk = NT >= 128;  // the CTA's tiles one after the other
   static constexpr int kTakeWarp0 = 4 * (1 + kUnpackWg);
   static constexpr int TC = NT / kTakeWg;           // rows per thread that holds sums
   static constexpr int kLaunch = NT <= 32 ? 40 : NT <= 64 ? 48 : 96;
@@ -169,21 +176,25 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
   constexpr int HS = S_::HS;
   extern __shared__ __align__(1024) uint8_t dsm[];
   __shared__ __align__(8) uint64_t full_w[kTqMaxW], empty_w[kTqMaxW], full_s[kTqMaxS],
-      empty_s[kTqMaxS], full_d[kTqMaxD], empty_d[kTqMaxD], done;
+      empty_s[kTqMaxS], full_d[S_::kD], empty_d[S_::kD], done;
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_bad;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int nkb = p.w.nkb, bb = p.w.block_bytes;
-  const int rank = blockIdx.x % c.cs, tile = blockIdx.x / c.cs, rt = blockIdx.y;
+  // this CTA's tiles: unit0, unit0 + step, ... (in a cluster one, shared)
+  const int rank = blockIdx.x % c.cs, unit0 = blockIdx.x / c.cs;
+  const int step = gridDim.x;
+  const int n_units = S_::kWalk && c.cs == 1 ? (c.units - unit0 + step - 1) / step : 1;
   const int kb0 = nkb * rank / c.cs, kb1 = nkb * (rank + 1) / c.cs;
-  const int blocks = kb1 - kb0, stages = blocks * 2 / HS;
+  const int blocks = kb1 - kb0, stages = blocks * 2 / HS;  // of a tile
   constexpr int kUnitB = NT * 128;  // a limb of a half
   const int stage_w = 2 * kQgQuad * bb;
-  // operand stage: HS halves of A, then [HS][limb] units of B
-  const int stage_s = HS * (kTqA + c.limbs * kUnitB);
+  // operand stage: [HS halves][limb] units of B (A's is in tensor memory)
+  const int stage_s = HS * c.limbs * kUnitB;
   uint8_t* ring_s = dsm;
   uint8_t* ring_w = dsm + c.nS * stage_s;
+  float* ring_o = reinterpret_cast<float*>(ring_w + c.nW * stage_w);  // result chunks, [warp][kChunk][kLdO]
   constexpr uint32_t kColsD = NT;
 
   if (threadIdx.x == 0) {
@@ -196,60 +207,73 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
       mbar_init(&full_s[s], 2 * HS * S_::kUnpackWg + 1);  // the unpacking warps, and the planes' bytes
       mbar_init(&empty_s[s], 1);
     }
-    for (int s = 0; s < c.nD; ++s) {
+    for (int s = 0; s < S_::kD; ++s) {
       mbar_init(&full_d[s], 1);
       mbar_init(&empty_d[s], 4 * S_::kTakeWg);
     }
     mbar_init(&done, 1);
     mbar_fence_init();
   }
-  // columns: a power of two of at least 32
-  uint32_t cols = 32;
-  while (cols < c.nD * kColsD) cols *= 2;
   if (warp == 1) {
-    tmem_alloc(&s_tmem, cols);
+    tmem_alloc(&s_tmem, S_::kCols);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = s_tmem;
+  const uint32_t tmem = s_tmem, tmem_a = tmem + S_::kD * NT;
   pdl_trigger();
 
   auto fail = [&]() {
     atomicOr(p.err, kErrWaitTimeout);
     s_bad = 1;
   };
-  // the tile's quads of columns (the second may not exist)
+  // a tile's quads of columns (the second may not exist)
   const size_t quad_bytes = (size_t)nkb * kQgQuad * bb;
-  const uint8_t* w0 = p.w.w + (size_t)tile * (p.w2 ? 1 : 2) * quad_bytes;
-  const uint8_t* w1 = p.w2 ? p.w2 + (size_t)tile * quad_bytes : w0 + quad_bytes;
-  const bool second = p.w2 || tile * 2 + 1 < q4g_quads(p.w.N);
+  const int quads = q4g_quads(p.w.N), run = kQgQuad * bb;
+  struct Unit {
+    int tile, rt;
+    const uint8_t *w0, *w1;
+    bool second;
+  };
+  auto unit = [&](int n) {
+    const int u = unit0 + n * step;
+    Unit o;
+    o.rt = u / c.tiles;
+    o.tile = u - o.rt * c.tiles;
+    o.w0 = p.w.w + (size_t)o.tile * (p.w2 ? 1 : 2) * quad_bytes + (size_t)kb0 * run;
+    o.w1 = p.w2 ? p.w2 + (size_t)o.tile * quad_bytes + (size_t)kb0 * run : o.w0 + quad_bytes;
+    o.second = p.w2 || o.tile * 2 + 1 < quads;
+    return o;
+  };
 
-  const int row0 = rt * NT, rows = min(NT, p.a.M - row0);
-  constexpr int kLd = 128 + 4;
-  float* S = reinterpret_cast<float*>(dsm);  // [NT][kLd]: staged sums
+  constexpr int kLd = 128 + 4, kLdO = kWarp + 4;
+  float* S = reinterpret_cast<float*>(dsm);  // [NT][kLd]: a cluster's staged sums
 
   if (warp < 4) {
     reg_dec<S_::kLow>();
     if (warp == 0) {
     // ------------------------------------------------ weight producer --
     if (lane == 0) {
-      const uint8_t* x0 = w0 + (size_t)kb0 * kQgQuad * bb;
-      const uint8_t* x1 = w1 + (size_t)kb0 * kQgQuad * bb;
-      const int n = blocks, run = kQgQuad * bb;
       Ring w;
       int i = 0;
-      for (; i < n; ++i, w.next(c.nW)) {  // no kernel writes the weights: no wait for the previous one
-        if (i >= c.nW && !mbar_wait(&empty_w[w.slot], w.phase ^ 1)) break;
-        uint8_t* st = ring_w + w.slot * stage_w;
-        mbar_expect_tx(&full_w[w.slot], run * (1 + second));
-        bulk_g2s(st, x0, run, &full_w[w.slot]);
-        if (second) bulk_g2s(st + run, x1, run, &full_w[w.slot]);
-        x0 += run;
-        x1 += run;
+      const int total = blocks * n_units;
+      for (int n = 0; n < n_units; ++n) {
+        const Unit t = unit(n);
+        const uint8_t *x0 = t.w0, *x1 = t.w1;
+        int b = 0;
+        for (; b < blocks; ++b, ++i, w.next(c.nW)) {  // no kernel writes the weights: no wait for the previous one
+          if (i >= c.nW && !mbar_wait(&empty_w[w.slot], w.phase ^ 1)) break;
+          uint8_t* st = ring_w + w.slot * stage_w;
+          mbar_expect_tx(&full_w[w.slot], run * (1 + t.second));
+          bulk_g2s(st, x0, run, &full_w[w.slot]);
+          if (t.second) bulk_g2s(st + run, x1, run, &full_w[w.slot]);
+          x0 += run;
+          x1 += run;
+        }
+        if (b < blocks) break;
       }
-      if (i < n) fail();
+      if (i < total) fail();
       // the copies issued last land before the CTA can exit
       for (int j = max(0, i - c.nW); j < i; ++j) mbar_wait(&full_w[j % c.nW], (j / c.nW) & 1);
     }
@@ -257,17 +281,22 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
     // ------------------------------------------------- planes producer --
     if (lane == 0) {
       const int bytes = HS * c.limbs * kUnitB;
-      const uint8_t* b0 = p.a.records + ((size_t)rt * nkb + kb0) * 2 * c.limbs * kUnitB;
       pdl_wait();
       Ring u;
       int i = 0;
-      for (; i < stages; ++i, u.next(c.nS)) {
-        if (i >= c.nS && !mbar_wait(&empty_s[u.slot], u.phase ^ 1)) break;
-        mbar_expect_tx(&full_s[u.slot], bytes);
-        bulk_g2s(ring_s + u.slot * stage_s + HS * kTqA, b0, bytes, &full_s[u.slot]);
-        b0 += bytes;
+      const int total = stages * n_units;
+      for (int n = 0; n < n_units; ++n) {
+        const uint8_t* b0 = p.a.records + ((size_t)unit(n).rt * nkb + kb0) * 2 * c.limbs * kUnitB;
+        int b = 0;
+        for (; b < stages; ++b, ++i, u.next(c.nS)) {
+          if (i >= c.nS && !mbar_wait(&empty_s[u.slot], u.phase ^ 1)) break;
+          mbar_expect_tx(&full_s[u.slot], bytes);
+          bulk_g2s(ring_s + u.slot * stage_s, b0, bytes, &full_s[u.slot]);
+          b0 += bytes;
+        }
+        if (b < stages) break;
       }
-      if (i < stages) {
+      if (i < total) {
         fail();
         // (the copies that were issued: bounded, the unpacking may have stopped)
         for (int j = max(0, i - c.nS); j < i; ++j) mbar_wait(&full_s[j % c.nS], (j / c.nS) & 1);
@@ -277,34 +306,21 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
     // ------------------------------------------------------ MMA issuer --
     // (the whole warp walks the loop, one lane issues)
     const uint32_t idesc = idesc_bf16(128, NT);
-    const uint64_t desc_a = umma_desc(smem_u32(ring_s), kTqLboA, 128);
-    const uint64_t desc_b = umma_desc(smem_u32(ring_s) + HS * kTqA, NT * 16, 128);
-    constexpr uint32_t kStepA = 2 * kTqLboA / 16, kStepB = 2 * NT;  // 16 k, in 16-byte units
+    const uint64_t desc_b = umma_desc_sw128(smem_u32(ring_s));
+    constexpr uint32_t kStepB = 2;  // 16 k, in 16-byte units
     // groups that a half completes (32: two, 64: one, 128: every second half one)
     constexpr int kSub = G == 1 ? 2 : 1, kK16 = 4 / kSub;
-    // a wait costs this warp as much as two MMAs, so those of the next stage are
-    // taken while half of this one's MMAs are still to issue; with an accumulator
-    // to wait for in every half that would hold MMAs back for the sums' warps
-    // (groups of 32, 2048 rows: 222 us, and 255 us so), so only for groups of 128
-    constexpr bool kAhead = G == 4;
     Ring rs, rd;
     int used = 0;  // accumulators begun
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t phase) {
       return __all_sync(0xffffffffu, mbar_wait(bar, phase)) != 0;
     };
-    // stage rs, and the accumulator rd if its first group begins one there
-    auto ready = [&](bool begins) {
-      return wait(&full_s[rs.slot], rs.phase) &&
-             (!begins || used < c.nD || wait(&empty_d[rd.slot], rd.phase ^ 1));
-    };
-    if (kAhead) ok = ready(true);
-    for (int j = 0; j < stages && ok; ++j) {
-      if (!kAhead) ok = wait(&full_s[rs.slot], rs.phase);
-      const uint64_t da = desc_a + (uint32_t)(rs.slot * stage_s / 16);
+    const int total = stages * n_units;  // (an even number of halves to a tile)
+    for (int j = 0; j < total && ok; ++j) {
+      ok = wait(&full_s[rs.slot], rs.phase);
+      const uint32_t da = tmem_a + (uint32_t)(rs.slot * HS * 32);
       const uint64_t db = desc_b + (uint32_t)(rs.slot * stage_s / 16);
-      const int slot = rs.slot;
-      rs.next(c.nS);
       tc_fence_after();
 #pragma unroll
       for (int h = 0; h < HS; ++h) {
@@ -312,44 +328,29 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
 #pragma unroll
         for (int g = 0; g < kSub; ++g) {
           const bool begins = G < 4 || !odd, ends = G < 4 || odd;
-          const bool last = h == HS - 1 && g == kSub - 1;
           if (begins) {
-            if (!kAhead && used >= c.nD) {
+            if (used >= S_::kD) {
               ok = ok && wait(&empty_d[rd.slot], rd.phase ^ 1);
               tc_fence_after();
             }
             ++used;
           }
           const uint32_t dt = tmem + (uint32_t)rd.slot * kColsD;
-          auto issue = [&](int l, int k) {
-            umma_bf16(dt, da + h * (kTqA / 16) + (g * kK16 + k) * kStepA,
-                      db + (uint32_t)((h * c.limbs + l) * (kUnitB / 16)) + (g * kK16 + k) * kStepB, idesc,
-                      k != 0 || l != 0 || !begins);
-          };
-          constexpr int kNow = kAhead ? kK16 / 2 : kK16;  // of a stage's last limb before the waits
           if (ok && elect_one()) {
-            for (int l = 0; l + 1 < c.limbs; ++l)
+            for (int l = 0; l < c.limbs; ++l)
 #pragma unroll
-              for (int k = 0; k < kK16; ++k) issue(l, k);
-#pragma unroll
-            for (int k = 0; k < (last ? kNow : kK16); ++k) issue(c.limbs - 1, k);
-            if ((!last || !kAhead) && ends) umma_commit(&full_d[rd.slot]);
-            if (last && !kAhead) umma_commit(&empty_s[slot]);
+              for (int k = 0; k < kK16; ++k)
+                umma_bf16_ta(dt, da + h * 32 + (g * kK16 + k) * 8,
+                             db + (uint32_t)((h * c.limbs + l) * (kUnitB / 16)) +
+                                 (g * kK16 + k) * kStepB,
+                             idesc, k != 0 || l != 0 || !begins);
+            if (ends) umma_commit(&full_d[rd.slot]);
+            if (h == HS - 1 && g == kSub - 1) umma_commit(&empty_s[rs.slot]);
           }
-          const int sd = rd.slot;
-          if (ends) rd.next(c.nD);
-          if (kAhead && last) {
-            const bool more = j + 1 >= stages || ready(HS == 2 || odd);
-            if (ok && elect_one()) {
-#pragma unroll
-              for (int k = kNow; k < kK16; ++k) issue(c.limbs - 1, k);
-              if (ends) umma_commit(&full_d[sd]);
-              umma_commit(&empty_s[slot]);
-            }
-            ok = ok && more;
-          }
+          if (ends) rd.next(S_::kD);
         }
       }
+      rs.next(c.nS);
     }
     if (!ok && lane == 0) fail();
     if (elect_one()) umma_commit(&done);  // arrives when every MMA issued above has finished
@@ -357,52 +358,66 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
     }
   } else if (warp < S_::kTakeWarp0) {
     // ----------------------------------------------------- unpacking --
-    // half of the warps the first half of each block, the others the second;
-    // kTiles neighbouring tiles to a warp
+    // half of the warps the first 64 k of each block, the others the second; of
+    // the 32 columns in the warp's quarter of the tensor memory's lanes, kTiles x 16
     reg_dec<S_::kLow>();
     constexpr int kTiles = 4 / S_::kUnpackWg;
-    const int half = (warp - 4) / (2 * S_::kUnpackWg), tile0 = (warp - 4) % (2 * S_::kUnpackWg) * kTiles;
-    const int r = lane >> 2, t = lane & 3;
-    const uint32_t ring_a = smem_u32(ring_s), ring_w_s = smem_u32(ring_w);
+    const int quad = warp & 3, wg = (warp - 4) >> 2;
+    const int half = wg * kTiles >> 1, j0 = kTiles == 1 ? wg & 1 : 0;
+    const int r = lane >> 2;
+    const uint32_t ring_w_s = smem_u32(ring_w);
+    const uint32_t ta = tmem_a + ((uint32_t)(quad * kWarp + j0 * 16) << 16) + (HS == 2 ? half * 32 : 0);
+    // the tiles among a stage's eight
+    const int piece = p.w2 ? quad + 4 * j0 : 2 * quad + j0, piece_step = (p.w2 ? 4 : 1) * bb;
     constexpr int ng = 4 / G;
-    const bool live = second || tile0 < 4;  // the tiles exist
     Ring rs, rw;
     if (HS == 1) rs.next(c.nS, half);
-    for (int kb = 0; kb < blocks; ++kb) {
-      if (!mbar_wait(&full_w[rw.slot], rw.phase)) {
-        if (lane == 0) fail();
-        break;
-      }
-      const uint32_t pc = ring_w_s + rw.slot * stage_w + tile0 * bb;
-      uint4 x[kTiles];
-      uint32_t z[kTiles][2];
+    int n = 0, left = blocks;
+    bool live = unit(0).second || quad < 2;  // the tiles exist
+    auto wait = [&](uint64_t* bar, uint32_t phase) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, phase)) != 0;
+    };
+    uint4 x[kTiles];
+    uint32_t z[kTiles][2];
+    auto load = [&]() {  // the tiles of the next block, if it has arrived
+      if (!wait(&full_w[rw.slot], rw.phase)) return false;
+      const uint32_t pc = ring_w_s + rw.slot * stage_w + piece * bb;
 #pragma unroll
       for (int j = 0; j < kTiles; ++j) {
-        x[j] = lds128(pc + j * bb + half * 512 + lane * 16);
+        x[j] = lds128(pc + j * piece_step + half * 512 + lane * 16);
         z[j][0] = z[j][1] = 0x0808u;
         if (p.w.zeros)
 #pragma unroll
           for (int hh = 0; hh < 2; ++hh)
-            z[j][hh] = lds16(pc + j * bb + kQgNibbles + ng * 32 + ((2 * half + hh) / G * 8 + r) * 2);
+            z[j][hh] = lds16(pc + j * piece_step + kQgNibbles + ng * 32 + ((2 * half + hh) / G * 8 + r) * 2);
       }
-      if ((HS == 1 ? 2 * kb + half : kb) >= c.nS && !mbar_wait(&empty_s[rs.slot], rs.phase ^ 1)) {
-        if (lane == 0) fail();
-        break;
+      return true;
+    };
+    bool ok = load();
+    const int total = blocks * n_units;
+    for (int kb = 0; kb < total && ok; ++kb, --left) {
+      if (left == 0) {
+        left = blocks;
+        live = unit(++n).second || quad < 2;
       }
+      ok = (HS == 1 ? 2 * kb + half : kb) < c.nS || wait(&empty_s[rs.slot], rs.phase ^ 1);
+      if (!ok) break;
+      tc_fence_after();
       if (live) {
-        const uint32_t dst = ring_a + rs.slot * stage_s + (HS == 2 ? half * kTqA : 0) + t * kTqLboA +
-                             tile0 * 256 + r * 16;
 #pragma unroll
         for (int j = 0; j < kTiles; ++j) {
           const uint32_t l0 = (0x4300u | (z[j][0] & 0xffu)) * 0x10001u, h0 = (0x4300u | (z[j][0] >> 8)) * 0x10001u;
           const uint32_t l1 = (0x4300u | (z[j][1] & 0xffu)) * 0x10001u, h1 = (0x4300u | (z[j][1] >> 8)) * 0x10001u;
-          sts128(dst + j * 256, unpack8(x[j].x, x[j].y, 0, l0));
-          sts128(dst + j * 256 + 128, unpack8(x[j].x, x[j].y, 4, h0));
-          sts128(dst + j * 256 + 4 * kTqLboA, unpack8(x[j].z, x[j].w, 0, l1));
-          sts128(dst + j * 256 + 4 * kTqLboA + 128, unpack8(x[j].z, x[j].w, 4, h1));
+          uint32_t o[16];
+          unpack8(x[j].x, x[j].y, 0, l0, o);
+          unpack8(x[j].x, x[j].y, 4, h0, o + 1);
+          unpack8(x[j].z, x[j].w, 0, l1, o + 8);
+          unpack8(x[j].z, x[j].w, 4, h1, o + 9);
+          tmem_st_16x32(ta + rs.slot * (HS * 32) + (j << 20), o);
         }
+        tmem_wait_st();
       }
-      fence_proxy_async_smem();
+      tc_fence_before();
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&full_s[rs.slot]);
@@ -413,98 +428,161 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
       }
       rw.next(c.nW);
       rs.next(c.nS, HS == 1 ? 2 : 1);
+      if (kb + 1 < total) ok = load();
     }
+    if (!ok && lane == 0) fail();
   } else {
     // ----------------------------------------------------- group sums --
     reg_inc<S_::kHigh>();
-    constexpr int TC = S_::TC;
+    constexpr int TC = S_::TC, kLoad = TC >= 64 ? 32 : 16;  // rows in all, and taken at once
     const int quad = warp & 3;                  // tensor-memory lanes 32 quad ..
     const int part = (warp - S_::kTakeWarp0) >> 2;  // rows part * TC ..
-    const int col = quad * kWarp + lane;        // the thread's weight column
-    float2 acc[TC / 2];
-#pragma unroll
-    for (int i = 0; i < TC / 2; ++i) acc[i] = make_float2(0.f, 0.f);
-    // the column's scales, a block ahead, from the weight's pieces (in L2)
+    // the thread's weight column: of this tile among a stage's eight (gated: of
+    // the gate for the lower lanes, the same column of the up weight for the others)
+    const int piece = p.w2 ? quad + (lane >> 4) * 4 : quad * 2 + (lane >> 4);
+    float* mine = ring_o + (warp - S_::kTakeWarp0) * kChunk * kLdO;
+    const int es = p.a.type == kQgF32 ? 4 : 2;
+    const bool plain = !p.accumulate && !((uintptr_t)p.out & 15) && p.ldo * es % 16 == 0;
     constexpr int ng = 4 / G;
-    const bool exists = second || quad < 2;
-    const uint8_t* scales = (quad < 2 ? w0 : w1) + (size_t)kb0 * kQgQuad * bb + ((col & 63) >> 4) * bb +
-                            kQgNibbles + ((col & 7) * 2 + ((col >> 3) & 1)) * 2;
-    unsigned short sn[ng];
-    auto fetch = [&]() {
-#pragma unroll
-      for (int g = 0; g < ng; ++g)
-        sn[g] = exists ? __ldg(reinterpret_cast<const unsigned short*>(scales + g * 32)) : 0;
-      scales += kQgQuad * bb;
-    };
-    fetch();
     Ring rd;
     bool ok = true;
-    for (int kb = 0; kb < blocks && ok; ++kb) {
-      float sc[ng];
+    float2 acc[TC / 2];
+    Unit un = unit(0);
+    for (int n_unit = 0; n_unit < n_units; ++n_unit) {
+      un = unit(n_unit);
+      const int row0 = un.rt * NT + part * TC, rows = p.a.M - row0;  // of this warp
 #pragma unroll
-      for (int g = 0; g < ng; ++g) sc[g] = u16_scale(sn[g], p.w.bf_scale);
-      if (kb + 1 < blocks) fetch();
-#pragma unroll
-      for (int g = 0; g < ng; ++g) {
-        ok = ok && mbar_wait(&full_d[rd.slot], rd.phase);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t ta = tmem + ((uint32_t)(quad * kWarp) << 16) + (uint32_t)(rd.slot * (int)kColsD + part * TC);
-        const float2 s2 = make_float2(sc[g], sc[g]);
-#pragma unroll
-        for (int i = 0; i < TC; i += 16) {
-          uint32_t v[16];
-          tmem_ld16(ta + i, v);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            fma2(acc[i / 2 + e], make_float2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), s2);
+      for (int i = 0; i < TC / 2; ++i) acc[i] = make_float2(0.f, 0.f);
+      // the column's scales, a block ahead, from the weight's pieces (in L2)
+      const bool exists = un.second || piece < 4;
+      const uint8_t* scales = (piece < 4 ? un.w0 : un.w1) + (piece & 3) * bb + kQgNibbles +
+                              ((lane & 7) * 2 + ((lane >> 3) & 1)) * 2;
+      uint2 sn = make_uint2(0, 0);  // the block's ng scales
+      auto fetch = [&]() {
+        const unsigned short* q = reinterpret_cast<const unsigned short*>(scales);
+        if (exists) {
+          sn.x = __ldg(q);
+          if (ng > 1) sn.x |= (uint32_t)__ldg(q + 16) << 16;
+          if (ng > 2) sn.y = __ldg(q + 32) | (uint32_t)__ldg(q + 48) << 16;
         }
-        tc_fence_before();
+        scales += run;
+      };
+      fetch();
+      for (int kb = 0; kb < blocks && ok; ++kb) {
+        uint2 sb = sn;
+        if (kb + 1 < blocks) fetch();
+#pragma unroll 1
+        for (int g = 0; g < ng; ++g) {
+          const float sc = u16_scale((unsigned short)(sb.x & 0xffffu), p.w.bf_scale);
+          sb.x = g == 1 ? sb.y : sb.x >> 16;
+          ok = ok && mbar_wait(&full_d[rd.slot], rd.phase);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t ta = tmem + ((uint32_t)(quad * kWarp) << 16) + (uint32_t)(rd.slot * (int)kColsD + part * TC);
+          const float2 s2 = make_float2(sc, sc);
+#pragma unroll
+          for (int i = 0; i < TC; i += kLoad) {
+            uint32_t v[kLoad / 16][16];
+#pragma unroll
+            for (int q = 0; q < kLoad / 16; ++q) tmem_ld16(ta + i + q * 16, v[q]);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < kLoad / 2; ++e)
+              fma2(acc[i / 2 + e],
+                   make_float2(__uint_as_float(v[e / 8][2 * (e & 7)]), __uint_as_float(v[e / 8][2 * (e & 7) + 1])), s2);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&empty_d[rd.slot]);
+          rd.next(S_::kD);
+        }
+      }
+      if (!S_::kWalk || c.cs > 1) break;
+      // ------------------------------------------------- a tile's results --
+      // through this warp's chunk of shared memory
+      ok = __all_sync(0xffffffffu, ok && !s_bad);
+      if (!ok) break;  // no results after a wait that ran out
+      if (n_unit == 0) pdl_wait();  // they may overwrite what the previous kernel still reads
+      const int n0 = un.tile * (p.w2 ? 64 : 128) + quad * (p.w2 ? kWarp / 2 : kWarp);  // first column
+      const bool fast = plain && n0 + kWarp <= p.w.N;
+#pragma unroll 1
+      for (int i = 0; i < TC; i += kChunk) {
+#pragma unroll
+        for (int h = 0; h < TC; h += kChunk)  // (the sums stay in registers)
+          if (h == i)
+#pragma unroll
+            for (int e = 0; e < kChunk; ++e)
+              mine[e * kLdO + lane] = e & 1 ? acc[(h + e) / 2].y : acc[(h + e) / 2].x;
         __syncwarp();
-        if (lane == 0) mbar_arrive(&empty_d[rd.slot]);
-        rd.next(c.nD);
+        const int e0 = lane >> 2, k4 = 4 * (lane & 3), k8 = 8 * (lane & 3);
+        if (p.w2) {
+#pragma unroll 2
+          for (int e = e0; e < kChunk; e += 8) {
+            const float* at = mine + e * kLdO + k4;
+            if (i + e < rows)
+              finish4(p, row0 + i + e, n0 + k4, *reinterpret_cast<const float4*>(at),
+                      *reinterpret_cast<const float4*>(at + 16));
+          }
+        } else if (fast) {
+#pragma unroll
+          for (int e = e0; e < kChunk; e += 8) {
+            const float* at = mine + e * kLdO + k8;
+            if (i + e < rows)
+              store8(p, row0 + i + e, n0 + k8, *reinterpret_cast<const float4*>(at),
+                     *reinterpret_cast<const float4*>(at + 4));
+          }
+        } else {
+#pragma unroll 1
+          for (int e = e0; e < kChunk && i + e < rows; e += 8)
+#pragma unroll 1
+            for (int k = k8; k < k8 + 8; k += 4) {
+              const float4 v = *reinterpret_cast<const float4*>(mine + e * kLdO + k);
+              finish4(p, row0 + i + e, n0 + k, v, v);
+            }
+        }
+        __syncwarp();
       }
     }
     if (!ok && lane == 0) fail();
     if (!mbar_wait(&done, 0) && lane == 0) fail();  // no MMA is in flight
     tc_fence_before();
     __syncthreads();
-    // --------------------------------------------------------- results --
+    if (S_::kWalk && c.cs == 1) return;
+    // -------------------------------- results of a CTA's, or cluster's, only tile --
     // by way of shared memory (every copy into it has landed: the MMAs and the
     // unpacking waited for them), rows of 128 columns, four to a thread
     int bad = s_bad;
+    const int rows = min(NT, p.a.M - un.rt * NT);
     pdl_wait();  // results may overwrite what the previous kernel still reads
 #pragma unroll
     for (int i = 0; i < TC; ++i)
-      S[(part * TC + i) * kLd + col] = i & 1 ? acc[i / 2].y : acc[i / 2].x;
+      S[(part * TC + i) * kLd + quad * kWarp + lane] = i & 1 ? acc[i / 2].y : acc[i / 2].x;
+    constexpr int kTakers = S_::kTakeWg * 4 * kWarp;
     if (c.cs > 1) {
       cluster_arrive();
       cluster_wait();
       const uint32_t bad0 = smem_u32(const_cast<int*>(&s_bad));
       for (int k = 0; k < c.cs; ++k) bad |= ld_dsmem_s32(dsmem_addr(bad0, (uint32_t)k));
     } else {
-      bar_sync_n(1, 4 * S_::kTakeWg * kWarp);
+      bar_sync_n(1, kTakers);
     }
     if (!bad) {  // no results after a wait that ran out
       const int out_cols = p.w2 ? 64 : 128, sh = p.w2 ? 4 : 5;
       // the rows of this rank, m = rank, rank + cs, ..., four columns to a thread
-      constexpr int kTakers = S_::kTakeWg * 4 * kWarp;
       const int i0 = threadIdx.x - S_::kTakeWarp0 * kWarp, n0 = 4 * (i0 & ((1 << sh) - 1));
-      const int step = (kTakers >> sh) * c.cs;
-#pragma unroll 2
-      for (int m = rank + (i0 >> sh) * c.cs; m < rows; m += step) {
+#pragma unroll 1
+      for (int m = rank + (i0 >> sh) * c.cs; m < rows; m += (kTakers >> sh) * c.cs) {
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f), u = v;
-        const float* at = S + m * kLd + n0;
+        const float* at = S + m * kLd + (p.w2 ? n0 + (n0 & ~15) : n0);
         if (c.cs > 1) {
           for (int k = 0; k < c.cs; ++k) add4(v, ld_dsmem4(dsmem_addr(smem_u32(at), (uint32_t)k)));
           if (p.w2)
-            for (int k = 0; k < c.cs; ++k) add4(u, ld_dsmem4(dsmem_addr(smem_u32(at + 64), (uint32_t)k)));
+            for (int k = 0; k < c.cs; ++k) add4(u, ld_dsmem4(dsmem_addr(smem_u32(at + 16), (uint32_t)k)));
         } else {
           v = *reinterpret_cast<const float4*>(at);
-          if (p.w2) u = *reinterpret_cast<const float4*>(at + 64);
+          if (p.w2) u = *reinterpret_cast<const float4*>(at + 16);
         }
-        finish4(p, row0 + m, tile * out_cols + n0, v, u);
+        finish4(p, un.rt * NT + m, un.tile * out_cols + n0, v, u);
       }
     }
     if (c.cs > 1) {  // the other CTAs have read this one's sums
@@ -516,7 +594,7 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
   // the other warps (few registers): the takers' barriers, and the tensor memory back
   __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, cols);
+  if (warp == 1) tmem_dealloc(tmem, S_::kCols);
   if (c.cs > 1) {
     cluster_arrive();
     cluster_wait();
@@ -527,6 +605,7 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
 
 struct TcPlan {
   int NT, tiles;
+  long long ctas;
   TcShape c;
   size_t smem;
 };
@@ -544,28 +623,27 @@ long long clusters_at_once(int sm_count, int ctas, int cs) {
 TcPlan plan_tc(const Q4gParams& p, int sm_count) {
   TcPlan o{};
   o.c.limbs = tc_limbs(p.a.type);
-  // rows per tile: as few tiles as fit (256 rows of one limb, 128 of more),
+  // rows per tile: as few tiles as fit (192 rows of one limb, 128 of more),
   // all of about the same size
-  const int most = o.c.limbs == 1 ? 256 : 128;
+  const int most = o.c.limbs == 1 ? 192 : 128;
   const int row_tiles = (p.a.M + most - 1) / most, each = (p.a.M + row_tiles - 1) / row_tiles;
-  const int sizes[5] = {32, 64, 128, 192, 256};
-  o.NT = 256;
-  // (with limbs a 32-row tile's stages leave one CTA to an SM: 24 rows fp32, K
-  // 2560, N 20480 took 62 us so and 50 us in tiles of 64)
-  for (int i = 4; i >= (o.c.limbs > 1 ? 1 : 0); --i)
+  const int sizes[4] = {32, 64, 128, 192};
+  for (int i = 3; i >= 0; --i)
     if (each <= sizes[i]) o.NT = sizes[i];
   o.c.row_tiles = (p.a.M + o.NT - 1) / o.NT;
   o.tiles = p.w2 ? q4g_quads(p.w.N) : (q4g_quads(p.w.N) + 1) / 2;
   // operand stages: at least two; what is left goes to them, then to the weights
-  const size_t limit = o.NT <= 64 ? kTqSmemMax / 2 : kTqSmemMax;
+  const size_t limit = o.NT <= 64 ? kTqSmemHalf : kTqSmemMax;
   const size_t stage_w = 2 * (size_t)kQgQuad * p.w.block_bytes;
-  const size_t stage_s = (o.NT <= 32 ? 2 : 1) * (kTqA + (size_t)o.c.limbs * o.NT * 128);
+  const size_t stage_s = (size_t)(o.NT == 32 || o.NT == 192 ? 2 : 1) * o.c.limbs * o.NT * 128;
   o.c.nS = 2;
   o.c.nW = 2;
-  o.c.nD = o.NT <= 128 ? 4 : 2;
-  size_t smem = o.c.nS * stage_s + o.c.nW * stage_w;
+  const int max_s = o.NT == 32 ? Tile<32>::kMaxS : o.NT == 64 ? Tile<64>::kMaxS : o.NT == 128 ? Tile<128>::kMaxS
+                                                                                 : Tile<192>::kMaxS;
+  const size_t chunks = o.NT >= 128 ? 8 * kChunk * (kWarp + 4) * sizeof(float) : 0;
+  size_t smem = o.c.nS * stage_s + o.c.nW * stage_w + chunks;
   const int ctas = smem <= limit && o.NT <= 64 ? 2 : 1;  // per SM
-  while (o.c.nS < kTqMaxS && smem + stage_s <= limit) {
+  while (o.c.nS < max_s && smem + stage_s <= limit) {
     ++o.c.nS;
     smem += stage_s;
   }
@@ -575,10 +653,12 @@ TcPlan plan_tc(const Q4gParams& p, int sm_count) {
   }
   const size_t staged = (size_t)o.NT * 132 * 4;
   o.smem = staged > smem ? staged : smem;
+  o.c.tiles = o.tiles;
+  o.c.units = o.tiles * o.c.row_tiles;
   // k shared by the CTAs of a cluster: the split with the least rounds x (blocks
   // of a CTA + what a CTA costs besides, about ten blocks).  A cluster's CTAs
   // share a GPC, so what fits at once is counted in clusters (16 rows, K 13824,
-  // N 5120: 40 clusters of seven do not, 39 us; of six they do, 29 us).
+  // N 5120: 40 clusters of seven do not, 36 us; of six they do, 27 us).
   const long long grid = (long long)o.tiles * o.c.row_tiles;
   long long best = 0;
   for (int cs = 1; cs <= kTqMaxCluster && (cs == 1 || p.w.nkb >= 4 * cs); ++cs) {
@@ -589,6 +669,9 @@ TcPlan plan_tc(const Q4gParams& p, int sm_count) {
       o.c.cs = cs;
     }
   }
+  const long long slots = clusters_at_once(sm_count, ctas, 1);
+  o.ctas = grid * o.c.cs;
+  if (o.NT >= 128 && o.c.cs == 1 && o.ctas > slots) o.ctas = slots;
   return o;
 }
 
@@ -596,7 +679,7 @@ template <int NT, int G>
 cudaError_t launch_tc_t(const Q4gParams& p, const TcPlan& o, cudaStream_t s) {
   if (o.smem > kTqSmemMax) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(o.tiles * o.c.cs, o.c.row_tiles, 1);
+  cfg.gridDim = dim3((unsigned)o.ctas, 1, 1);
   cfg.blockDim = dim3(Tile<NT>::kThreads);
   cfg.dynamicSmemBytes = o.smem;
   cfg.stream = s;
@@ -624,27 +707,27 @@ cudaError_t launch_tc_g(const Q4gParams& p, const TcPlan& o, cudaStream_t s) {
   }
 }
 
-template <int NT>
-void count_clusters(int ctas) {
-  for (int cs = kTqMaxCluster; cs >= 1; --cs) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(cs * 1024);
-    cfg.blockDim = dim3(Tile<NT>::kThreads);
-    cfg.dynamicSmemBytes = kTqSmemMax / ctas;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)cs;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, q4g_tc_kernel<NT, 4>, &cfg) != cudaSuccess) {
-      cudaGetLastError();
-      n = 0;
+// Asked with a kernel that has no tensor memory: of one that has, the runtime
+// counts one CTA to an SM, while two whose columns fit do run together.
+cudaError_t count_clusters() {
+  cudaError_t e = cudaFuncSetAttribute(q4g_planes_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)kTqSmemMax);
+  for (int ctas = 1; ctas <= 2 && e == cudaSuccess; ++ctas)
+    for (int cs = kTqMaxCluster; cs >= 1 && e == cudaSuccess; --cs) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(cs * 1024);
+      cfg.blockDim = dim3(128);
+      cfg.dynamicSmemBytes = ctas == 2 ? kTqSmemHalf : kTqSmemMax;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = (unsigned)cs;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      e = cudaOccupancyMaxActiveClusters(&g_clusters[ctas][cs], q4g_planes_kernel, &cfg);
     }
-    g_clusters[ctas][cs] = n;
-  }
+  return e;
 }
 
 template <int NT, int G>
@@ -671,8 +754,8 @@ cudaError_t launch_q4g_tc(const Q4gParams& p, int sm_count, cudaStream_t s) {
   const TcPlan o = plan_tc(p, sm_count);
   const int m8 = (p.a.M + 7) / 8;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((p.w.nkb * 16 + 31) / 32, m8 < 65535 ? m8 : 65535, 1);
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3((p.w.nkb * 4 + 15) / 16, m8 < 65535 ? m8 : 65535, 1);
+  cfg.blockDim = dim3(128);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -686,8 +769,7 @@ cudaError_t launch_q4g_tc(const Q4gParams& p, int sm_count, cudaStream_t s) {
     case 64: return launch_tc_g<64>(p, o, s);
     case 128: return launch_tc_g<128>(p, o, s);
     case 192: return launch_tc_g<192>(p, o, s);
-    case 256: return launch_tc_g<256>(p, o, s);
-  }
+      }
   return cudaErrorInvalidValue;
 }
 
@@ -696,11 +778,7 @@ cudaError_t prepare_q4g_tc() {
   if (e == cudaSuccess) e = prepare_tc_g<64>();
   if (e == cudaSuccess) e = prepare_tc_g<128>();
   if (e == cudaSuccess) e = prepare_tc_g<192>();
-  if (e == cudaSuccess) e = prepare_tc_g<256>();
-  if (e == cudaSuccess && !g_clusters[1][1]) {  // (every GPU of a node is alike)
-    count_clusters<64>(2);
-    count_clusters<256>(1);
-  }
+  if (e == cudaSuccess && !g_clusters[1][1]) e = count_clusters();  // (every GPU of a node is alike)
   return e;
 }
 
