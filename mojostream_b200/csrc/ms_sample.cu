@@ -300,6 +300,7 @@ __global__ void __launch_bounds__(kSampThreads) sample_kernel(const SampleParams
       float bv = -INFINITY;
       int bi = INT_MAX;
       for (int c = 0; c < p.nchunk; ++c) first_max(bv, bi, sh.part[c].x, __float_as_int(sh.part[c].y));
+      if (bi == INT_MAX) bi = 0;  // nothing above -inf in the row: its first id
       if (p.maxval) {  // tensor parallel: local index + value, combined over ranks
         p.maxval[r] = bv;
         p.out[r] = bi;
