@@ -163,12 +163,19 @@ MS_API size_t ms_q4g_weight_bytes(const ms_q4g_weight *w);
 /* C[M,N] = A[M,K] . w (accumulate = 0) or C += A . w (accumulate = 1).
  * A and C: device memory of one type (dtype), rows lda >= K and ldc >= N
  * elements apart, aligned to their elements; they must not share memory.
- * Activations are used exactly as given and sums are fp32, rounded once to
- * dtype.  The call uses the context's workspace (rows of 16-bit limbs,
- * M * K * 2 bytes per limb; 3 limbs for fp32, 2 for half, 1 for bfloat16):
- * it grows on the first call of a size, which must not happen inside a
- * stream capture (MS_ERR_STATE), and calls on different streams must not
- * overlap in time, captured and replayed ones included. */
+ * M <= 4194304.  Sums are fp32, rounded once to dtype.
+ *   Few rows (up to 8 of bfloat16, 16 of fp32 and half): a value is held to
+ * 2^-30 (fp32) or 2^-22 of the largest of its group in its row, at least
+ * 2^-120.  More rows: values are used exactly as given.  A group whose sum
+ * passes the range of fp32 before its scale is applied (magnitudes near 2^117
+ * and up) overflows to infinity or NaN; an infinity or NaN in a row of A makes
+ * that row's results infinite or NaN, and no other row's.
+ *   The call may use the context's workspace: for each value of A (k rounded
+ * up to 128) at most 5 bytes with few rows, rounded up to 8; 2 (bfloat16), 4
+ * (half) or 6 (fp32) bytes with more, rounded up to whole tiles of 32 to 192.
+ * It grows on the first call of a size, which must not happen inside a stream
+ * capture (MS_ERR_STATE), and calls on different streams must not overlap in
+ * time, captured and replayed ones included. */
 MS_API ms_status ms_q4g_gemm(ms_ctx *ctx, const ms_q4g_weight *w, void *C, int64_t ldc,
                       const void *A, int64_t lda, int dtype, int M, int accumulate,
                       void *stream);

@@ -101,9 +101,10 @@ cudaError_t launch_q4g_stream(const Q4gParams& p, int sm_count, cudaStream_t s);
 cudaError_t prepare_q4g();
 // Many rows on tcgen05 (ms_q4g_tc.cu): two launches; p.a.records is workspace
 // of q4g_planes_bytes.
-// From how many rows on: 9 bfloat16 rows (K 13824, N 5120: 32 us, two rounds of
-// the streaming kernel 37 us; at 24 rows 33 and 50 us), 17 rows that take two or
-// three limbs (K 5120, N 13824 fp32: 16 rows 48 and 36 us, 32 rows 48 and 66 us).
+// From how many rows on: 9 bfloat16 rows (K 13824, N 5120: 27 us, two rounds of
+// the streaming kernel 37 us; 8 rows 27 and 27 us), 17 rows that take two or
+// three limbs (K 2560, N 20480 half: 16 rows 29 and 27 us, 20 rows 29 and 35 us;
+// K 5120, N 13824 fp32: 34 and 36, 34 and 50 us).
 inline int q4g_tc_rows(int type) { return type == kQgBf16 ? 9 : 17; }
 size_t q4g_planes_bytes(const Q4gParams& p, int sm_count);
 cudaError_t launch_q4g_tc(const Q4gParams& p, int sm_count, cudaStream_t s);

@@ -27,11 +27,15 @@
 // next tile are there when it begins.  Where there are too few tiles, a
 // cluster's CTAs share the k of one; their sums are added in k order through
 // distributed shared memory.
-// Every role's loop shares the SM's instruction cache with the others, and its
-// length is what bounds them: with unrolled limbs and the next stage's waits
-// among the MMAs 2048 rows (K 2560, N 10240, bfloat16) took 137 us, and take
-// 103 us (1045 TFLOP/s; 4096 x 5120 x 13824 593 us, 978 TFLOP/s), with the
+// The loops are kept short: with unrolled limbs and the next stage's waits among
+// the MMAs 2048 rows (K 2560, N 10240, bfloat16) took 137 us, and take 103 us
+// (1045 TFLOP/s; 4096 x 5120 x 13824 574 us, 1010 TFLOP/s), with the
 // activation's exact division unrolled 519 gated rows took 114 us, and take 98.
+//
+// What bounds it: many rows, the operands' way from L2, 58 KB a block in about
+// 1000 cycles of a port of 64 bytes (2048 rows without any MMA or tensor memory
+// traffic: 93 us); few rows, the instructions that unpack (64 gated rows, K
+// 5120, N 13824: 52 us, without them 42 us).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -642,7 +646,7 @@ TcPlan plan_tc(const Q4gParams& p, int sm_count) {
                                                                                  : Tile<192>::kMaxS;
   const size_t chunks = o.NT >= 128 ? 8 * kChunk * (kWarp + 4) * sizeof(float) : 0;
   size_t smem = o.c.nS * stage_s + o.c.nW * stage_w + chunks;
-  const int ctas = smem <= limit && o.NT <= 64 ? 2 : 1;  // per SM
+  const int ctas = o.NT <= 64 ? 2 : 1;  // per SM
   while (o.c.nS < max_s && smem + stage_s <= limit) {
     ++o.c.nS;
     smem += stage_s;
@@ -651,8 +655,13 @@ TcPlan plan_tc(const Q4gParams& p, int sm_count) {
     ++o.c.nW;
     smem += stage_w;
   }
-  const size_t staged = (size_t)o.NT * 132 * 4;
-  o.smem = staged > smem ? staged : smem;
+  // All of it, so that no CTA of another kernel that needs more tensor memory
+  // than is left can share the SM: two clusters whose CTAs waited there for each
+  // other's tensor memory would not end.
+  o.smem = smem <= limit ? limit : 0;
+  static_assert((size_t)Tile<192>::kTakeWg * Tile<192>::TC * 132 * 4 <= kTqSmemMax &&
+                    (size_t)Tile<64>::kTakeWg * Tile<64>::TC * 132 * 4 <= kTqSmemHalf,
+                "a cluster's staged sums");
   o.c.tiles = o.tiles;
   o.c.units = o.tiles * o.c.row_tiles;
   // k shared by the CTAs of a cluster: the split with the least rounds x (blocks
@@ -677,7 +686,7 @@ TcPlan plan_tc(const Q4gParams& p, int sm_count) {
 
 template <int NT, int G>
 cudaError_t launch_tc_t(const Q4gParams& p, const TcPlan& o, cudaStream_t s) {
-  if (o.smem > kTqSmemMax) return cudaErrorInvalidConfiguration;
+  if (!o.smem) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)o.ctas, 1, 1);
   cfg.blockDim = dim3(Tile<NT>::kThreads);
