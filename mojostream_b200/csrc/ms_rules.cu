@@ -13,10 +13,11 @@
 // lists name are rewritten one by one afterwards.
 //   Few columns in all: one kernel, whose CTAs count the history's ids of their
 // columns in shared memory while their pieces are on the way (one row, V
-// 262144: 4.2 us).  Many: every CTA would scan its row's history for a sliver
-// of columns (64 rows, 4096 ids: 44 us against 28 us for the stream alone), so
-// the stream runs by itself and a second kernel, which starts as the first
-// drains, gathers each row's ids in hash tables and rewrites them.
+// 262144: 4.1 us).  Many: every CTA would scan its row's history for a sliver
+// of columns, so the stream runs by itself and a second kernel, which starts as
+// the first drains, gathers each row's ids in hash tables and rewrites them (64
+// rows of V 262144, 4096 ids each, 16 masks: 39 us in one kernel, 26 us in two,
+// of them 22 us the stream, 4.5 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
