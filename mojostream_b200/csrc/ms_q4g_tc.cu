@@ -2,8 +2,10 @@
 // the 5th-generation tensor cores (layout: ms_q4g.h):
 //   C[m][n] (+)= sum_k A[m][k] (q[k][n] - z) s,   H = act(A Wg) * (A Wu).
 //
-// Mathematics.  q - z is an integer of at most 5 bits: exact in bfloat16
-// ((0x4300 | q) is the bfloat16 128 + q; subtracting 128 + z leaves q - z).
+// Mathematics.  q - z is an integer of at most 5 bits: exact in bfloat16.  The
+// bits of q alone, in bits 0-3 or 4-7, are the bfloat16 q 2^-133 or 16 q 2^-133
+// (the numbers up to 2^-125 are evenly spaced), so one fused multiply-add gives
+// (q - z) / 128 without a shift; the sums are multiplied by 128 at the end.
 // An activation is cut into bfloat16 limbs that add up to it exactly (fp32:
 // 8 + 8 + 8 bits, fp16: 8 + 3, bfloat16: itself), so every product of a
 // tcgen05.mma is exact and its fp32 accumulator in tensor memory holds the sum
@@ -120,13 +122,26 @@ struct TcShape {
   int tiles, units;  // column tiles; tiles in all
 };
 
-// Four bfloat16 pairs of one column, k 0..7 of the words x, y, into every other of r.
-__device__ __forceinline__ void unpack8(uint32_t x, uint32_t y, int shift, uint32_t bias, uint32_t* r) {
-  const uint32_t w[4] = {x >> shift, x >> (8 + shift), y >> shift, y >> (8 + shift)};
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+constexpr uint32_t kUp126 = 0x7E807E80u, kUp122 = 0x7C807C80u;  // pairs of 2^126, 2^122
+constexpr uint32_t kMinus8 = 0xBD80BD80u;                       // -8 / 128
+// -z / 128 in both halves, z a byte of v (0 or 1)
+__device__ __forceinline__ uint32_t bias_of(uint32_t v, int byte) {
+  return fma_bf16x2(__byte_perm(v, 0, byte ? 0x4141 : 0x4040), kUp126 | 0x80008000u, 0x80008000u);
+}
+// k 0..7 of the columns r (low nibbles) and r + 8 in the words x, y as bfloat16
+// pairs: r's into the even, the other's into the odd of o.
+__device__ __forceinline__ void unpack16(uint32_t x, uint32_t y, uint32_t bias_lo, uint32_t bias_hi,
+                                         uint32_t* o) {
+  const uint32_t w[4] = {x, x >> 8, y, y >> 8};
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const uint32_t v = (w[e] & 0x000F000Fu) | 0x43004300u;
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r[2 * e]) : "r"(v), "r"(bias));
+    o[2 * e] = fma_bf16x2(w[e] & 0x000F000Fu, kUp126, bias_lo);
+    o[2 * e + 1] = fma_bf16x2(w[e] & 0x00F000F0u, kUp122, bias_hi);
   }
 }
 // One lane of a converged warp, the same on every call: the compiler then
@@ -389,7 +404,6 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
 #pragma unroll
       for (int j = 0; j < kTiles; ++j) {
         x[j] = lds128(pc + j * piece_step + half * 512 + lane * 16);
-        z[j][0] = z[j][1] = 0x0808u;
         if (p.w.zeros)
 #pragma unroll
           for (int hh = 0; hh < 2; ++hh)
@@ -410,13 +424,14 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
       if (live) {
 #pragma unroll
         for (int j = 0; j < kTiles; ++j) {
-          const uint32_t l0 = (0x4300u | (z[j][0] & 0xffu)) * 0x10001u, h0 = (0x4300u | (z[j][0] >> 8)) * 0x10001u;
-          const uint32_t l1 = (0x4300u | (z[j][1] & 0xffu)) * 0x10001u, h1 = (0x4300u | (z[j][1] >> 8)) * 0x10001u;
           uint32_t o[16];
-          unpack8(x[j].x, x[j].y, 0, l0, o);
-          unpack8(x[j].x, x[j].y, 4, h0, o + 1);
-          unpack8(x[j].z, x[j].w, 0, l1, o + 8);
-          unpack8(x[j].z, x[j].w, 4, h1, o + 9);
+          if (p.w.zeros) {
+            unpack16(x[j].x, x[j].y, bias_of(z[j][0], 0), bias_of(z[j][0], 1), o);
+            unpack16(x[j].z, x[j].w, bias_of(z[j][1], 0), bias_of(z[j][1], 1), o + 8);
+          } else {
+            unpack16(x[j].x, x[j].y, kMinus8, kMinus8, o);
+            unpack16(x[j].z, x[j].w, kMinus8, kMinus8, o + 8);
+          }
           tmem_st_16x32(ta + rs.slot * (HS * 32) + (j << 20), o);
         }
         tmem_wait_st();
@@ -516,7 +531,7 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
           if (h == i)
 #pragma unroll
             for (int e = 0; e < kChunk; ++e)
-              mine[e * kLdO + lane] = e & 1 ? acc[(h + e) / 2].y : acc[(h + e) / 2].x;
+              mine[e * kLdO + lane] = 128.f * (e & 1 ? acc[(h + e) / 2].y : acc[(h + e) / 2].x);
         __syncwarp();
         const int e0 = lane >> 2, k4 = 4 * (lane & 3), k8 = 8 * (lane & 3);
         if (p.w2) {
@@ -560,7 +575,7 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
     pdl_wait();  // results may overwrite what the previous kernel still reads
 #pragma unroll
     for (int i = 0; i < TC; ++i)
-      S[(part * TC + i) * kLd + quad * kWarp + lane] = i & 1 ? acc[i / 2].y : acc[i / 2].x;
+      S[(part * TC + i) * kLd + quad * kWarp + lane] = 128.f * (i & 1 ? acc[i / 2].y : acc[i / 2].x);
     constexpr int kTakers = S_::kTakeWg * 4 * kWarp;
     if (c.cs > 1) {
       cluster_arrive();
