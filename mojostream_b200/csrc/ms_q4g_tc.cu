@@ -30,14 +30,15 @@
 // cluster's CTAs share the k of one; their sums are added in k order through
 // distributed shared memory.
 // The loops are kept short: with unrolled limbs and the next stage's waits among
-// the MMAs 2048 rows (K 2560, N 10240, bfloat16) took 137 us, and take 103 us
-// (1045 TFLOP/s; 4096 x 5120 x 13824 574 us, 1010 TFLOP/s), with the
-// activation's exact division unrolled 519 gated rows took 114 us, and take 98.
+// the MMAs 2048 rows (K 2560, N 10240, bfloat16) took 137 us, and take 99 us
+// (1085 TFLOP/s; 4096 x 5120 x 13824 537 us, 1080 TFLOP/s), with the
+// activation's exact division unrolled 519 gated rows took 114 us, and take 97.
 //
-// What bounds it: many rows, the operands' way from L2, 58 KB a block in about
-// 1000 cycles of a port of 64 bytes (2048 rows without any MMA or tensor memory
-// traffic: 93 us); few rows, the instructions that unpack (64 gated rows, K
-// 5120, N 13824: 52 us, without them 42 us).
+// What bounds it: many rows, the MMAs (at their measured rate 65 of the 99 us)
+// and the hand-over between the roles; a quarter of the planes' bytes (58 KB a
+// block come from L2) would save 9 us, no writing of results as much.  Few rows:
+// the instructions that unpack (64 gated rows, K 5120, N 13824: 52 us; 42 us
+// without those that shifted and subtracted, a third of which is gone since).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -144,6 +145,17 @@ __device__ __forceinline__ void unpack16(uint32_t x, uint32_t y, uint32_t bias_l
     o[2 * e + 1] = fma_bf16x2(w[e] & 0x00F000F0u, kUp122, bias_hi);
   }
 }
+// Shared to global, both 16-byte aligned, in the thread's open bulk group.
+__device__ __forceinline__ void bulk_s2g(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void sts16(uint32_t a, uint32_t v) {
+  asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"((unsigned short)v) : "memory");
+}
 // One lane of a converged warp, the same on every call: the compiler then
 // keeps what that lane hands to the tensor core in uniform registers (behind
 // lane == 0 an MMA took 125 cycles to issue).
@@ -195,7 +207,7 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
   constexpr int HS = S_::HS;
   extern __shared__ __align__(1024) uint8_t dsm[];
   __shared__ __align__(8) uint64_t full_w[kTqMaxW], empty_w[kTqMaxW], full_s[kTqMaxS],
-      empty_s[kTqMaxS], full_d[S_::kD], empty_d[S_::kD], done;
+      empty_s[kTqMaxS], full_d[S_::kD], empty_d[S_::kD], done, full_t, empty_t;
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_bad;
 
@@ -213,7 +225,8 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
   const int stage_s = HS * c.limbs * kUnitB;
   uint8_t* ring_s = dsm;
   uint8_t* ring_w = dsm + c.nS * stage_s;
-  float* ring_o = reinterpret_cast<float*>(ring_w + c.nW * stage_w);  // result chunks, [warp][kChunk][kLdO]
+  float* ring_o = reinterpret_cast<float*>(ring_w + c.nW * stage_w);  // results: a tile of 16-bit
+                                                                     // rows, or [warp][kChunk][kLdO]
   constexpr uint32_t kColsD = NT;
 
   if (threadIdx.x == 0) {
@@ -231,6 +244,8 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
       mbar_init(&empty_d[s], 4 * S_::kTakeWg);
     }
     mbar_init(&done, 1);
+    mbar_init(&full_t, 4 * S_::kTakeWg);
+    mbar_init(&empty_t, 1);
     mbar_fence_init();
   }
   if (warp == 1) {
@@ -264,6 +279,15 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
     o.w1 = p.w2 ? p.w2 + (size_t)o.tile * quad_bytes + (size_t)kb0 * run : o.w0 + quad_bytes;
     o.second = p.w2 || o.tile * 2 + 1 < quads;
     return o;
+  };
+
+  // a tile whose results leave by bulk copies while the next one is made: not
+  // the last, only rounded, inside the matrix, aligned (2048 rows: 104 us without,
+  // and 99 us; the last tile so, too: 128 rows, K 5120, N 13824 38 and 41 us)
+  const bool plain = S_::kWalk && c.cs == 1 && !p.accumulate && !p.w2 && !((uintptr_t)p.out & 15) &&
+                     p.ldo * (p.a.type == kQgF32 ? 4 : 2) % 16 == 0;
+  auto by_bulk = [&](const Unit& t, int n) {
+    return plain && p.a.type != kQgF32 && n + 1 < n_units && t.tile * 128 + 128 <= p.w.N;
   };
 
   constexpr int kLd = 128 + 4, kLdO = kWarp + 4;
@@ -374,6 +398,27 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
     if (!ok && lane == 0) fail();
     if (elect_one()) umma_commit(&done);  // arrives when every MMA issued above has finished
     __syncwarp();
+    } else if (plain) {
+    // ------------------------------------- whole tiles of 16-bit results --
+    pdl_wait();  // they may overwrite what the previous kernel still reads
+    int written = 0;
+    for (int n = 0; n < n_units; ++n) {
+      const Unit t = unit(n);
+      if (!by_bulk(t, n)) continue;
+      if (!__all_sync(0xffffffffu, mbar_wait(&full_t, written & 1))) {
+        if (lane == 0) fail();
+        break;
+      }
+      const int rows = min(NT, p.a.M - t.rt * NT);
+      uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) + ((size_t)t.rt * NT * p.ldo + t.tile * 128) * 2;
+      for (int r = lane; r < rows; r += kWarp) bulk_s2g(dst + (size_t)r * p.ldo * 2, smem_u32(ring_o) + r * 256, 256);
+      bulk_commit();
+      bulk_wait_read();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty_t);
+      ++written;
+    }
+    bulk_wait();
     }
   } else if (warp < S_::kTakeWarp0) {
     // ----------------------------------------------------- unpacking --
@@ -460,8 +505,7 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
     // the gate for the lower lanes, the same column of the up weight for the others)
     const int piece = p.w2 ? quad + (lane >> 4) * 4 : quad * 2 + (lane >> 4);
     float* mine = ring_o + (warp - S_::kTakeWarp0) * kChunk * kLdO;
-    const int es = p.a.type == kQgF32 ? 4 : 2;
-    const bool plain = !p.accumulate && !((uintptr_t)p.out & 15) && p.ldo * es % 16 == 0;
+    int written = 0;  // tiles by bulk copies
     constexpr int ng = 4 / G;
     Ring rd;
     bool ok = true;
@@ -524,6 +568,29 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
       if (n_unit == 0) pdl_wait();  // they may overwrite what the previous kernel still reads
       const int n0 = un.tile * (p.w2 ? 64 : 128) + quad * (p.w2 ? kWarp / 2 : kWarp);  // first column
       const bool fast = plain && n0 + kWarp <= p.w.N;
+      if (written > 0 && !__all_sync(0xffffffffu, mbar_wait(&empty_t, (written - 1) & 1))) {
+        ok = false;
+        break;
+      }
+      if (by_bulk(un, n_unit)) {
+        const uint32_t at = smem_u32(ring_o) + part * TC * 256 + (quad * kWarp + lane) * 2;
+#pragma unroll
+        for (int i = 0; i < TC; i += 2) {
+          const float lo = 128.f * acc[i / 2].x, hi = 128.f * acc[i / 2].y;
+          uint32_t v;
+          if (p.a.type == kQgBf16)
+            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
+          else
+            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
+          sts16(at + i * 256, v);
+          sts16(at + i * 256 + 256, v >> 16);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full_t);
+        ++written;
+        continue;
+      }
 #pragma unroll 1
       for (int i = 0; i < TC; i += kChunk) {
 #pragma unroll
@@ -659,7 +726,8 @@ TcPlan plan_tc(const Q4gParams& p, int sm_count) {
   o.c.nW = 2;
   const int max_s = o.NT == 32 ? Tile<32>::kMaxS : o.NT == 64 ? Tile<64>::kMaxS : o.NT == 128 ? Tile<128>::kMaxS
                                                                                  : Tile<192>::kMaxS;
-  const size_t chunks = o.NT >= 128 ? 8 * kChunk * (kWarp + 4) * sizeof(float) : 0;
+  size_t chunks = o.NT >= 128 ? 8 * kChunk * (kWarp + 4) * sizeof(float) : 0;
+  if (o.NT >= 128 && o.c.limbs < 3 && chunks < (size_t)o.NT * 256) chunks = (size_t)o.NT * 256;
   size_t smem = o.c.nS * stage_s + o.c.nW * stage_w + chunks;
   const int ctas = o.NT <= 64 ? 2 : 1;  // per SM
   while (o.c.nS < max_s && smem + stage_s <= limit) {
