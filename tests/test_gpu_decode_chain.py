@@ -6,7 +6,8 @@ import pytest
 
 from mojostream_b200.model import small_spec, synth_weights
 from rules_check import reference, words
-from test_gpu_q4g import bound, dense, gated_exact, make_weight, rounded, sums_bound, U
+from test_gpu_q4g import U, bound, check, dense, gated_exact, make_weight, rounded, sums_bound
+from test_gpu_q4g import test_gated as gated_case
 
 pytestmark = pytest.mark.gpu
 
@@ -155,3 +156,22 @@ def test_back_to_back(ctx, torch_cuda, op, M, K, N, g, zeros, dtype):
         torch.cuda.synchronize()
         for j, c in enumerate(cs):
             assert torch.equal(c, alone[j % 2]), j
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("pad,accumulate", [
+    (7, False),  # rows of the result start on 16-byte boundaries
+    (2, False),  # and do not
+    (7, True),
+])
+def test_more_tiles_than_sms(ctx, torch_cuda, dtype, pad, accumulate):
+    """A CTA makes several tiles: whole ones, one whose columns end inside it
+    and rows that do, against the definition."""
+    check(torch_cuda, ctx, 1100, 256, 5136, 64, not accumulate, getattr(torch_cuda, dtype), pad,
+          accumulate=accumulate)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("N,pad", [(3000, 7), (3010, 2)])
+def test_more_gated_tiles_than_sms(ctx, torch_cuda, dtype, N, pad):
+    gated_case(ctx, torch_cuda, 700, 256, N, 32, True, pad, "silu", dtype)
