@@ -51,11 +51,12 @@
 namespace ms {
 namespace {
 
-constexpr int kTqMaxS = 4, kTqMaxW = 8, kTqMaxD = 3;
+constexpr int kTqMaxS = 4, kTqMaxW = 8;
 // dynamic shared memory of a CTA, alone on its SM or one of two
 constexpr size_t kTqSmemMax = 224 * 1024, kTqSmemHalf = 110 * 1024;
 constexpr int kTqMaxCluster = 8;
 constexpr int kChunk = 32;  // rows of a chunk of results
+constexpr int kChunkBytes = 8 * kChunk * (kWarp + 4) * 4;
 
 // -------------------------------------------------------------- planes --
 // The next limb of v, the leading 8 bits of what is left (truncated, so nothing
@@ -180,7 +181,7 @@ struct Tile {
   static constexpr int kCols = 512 / kCtas;
   static constexpr int kD = NT == 128 ? 3 : 2;
   static constexpr int kMaxS = (kCols - kD * NT) / (32 * HS);
-  static_assert(kD <= kTqMaxD && kMaxS >= 2, "tensor memory");
+  static_assert(kMaxS >= 2 && kMaxS <= kTqMaxS, "tensor memory");
   static constexpr bool kWalk = NT >= 128;  // the CTA's tiles one after the other
   static constexpr int kTakeWarp0 = 4 * (1 + kUnpackWg);
   static constexpr int TC = NT / kTakeWg;           // rows per thread that holds sums
@@ -225,8 +226,10 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
   const int stage_s = HS * c.limbs * kUnitB;
   uint8_t* ring_s = dsm;
   uint8_t* ring_w = dsm + c.nS * stage_s;
-  float* ring_o = reinterpret_cast<float*>(ring_w + c.nW * stage_w);  // results: a tile of 16-bit
-                                                                     // rows, or [warp][kChunk][kLdO]
+  // results: [warp][kChunk][kLdO], and behind them a tile of 16-bit rows (apart:
+  // a warp may be a tile ahead of another)
+  float* ring_o = reinterpret_cast<float*>(ring_w + c.nW * stage_w);
+  const uint32_t tile_o = smem_u32(ring_o) + kChunkBytes;
   constexpr uint32_t kColsD = NT;
 
   if (threadIdx.x == 0) {
@@ -411,7 +414,7 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
       }
       const int rows = min(NT, p.a.M - t.rt * NT);
       uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) + ((size_t)t.rt * NT * p.ldo + t.tile * 128) * 2;
-      for (int r = lane; r < rows; r += kWarp) bulk_s2g(dst + (size_t)r * p.ldo * 2, smem_u32(ring_o) + r * 256, 256);
+      for (int r = lane; r < rows; r += kWarp) bulk_s2g(dst + (size_t)r * p.ldo * 2, tile_o + r * 256, 256);
       bulk_commit();
       bulk_wait_read();
       __syncwarp();
@@ -568,12 +571,12 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
       if (n_unit == 0) pdl_wait();  // they may overwrite what the previous kernel still reads
       const int n0 = un.tile * (p.w2 ? 64 : 128) + quad * (p.w2 ? kWarp / 2 : kWarp);  // first column
       const bool fast = plain && n0 + kWarp <= p.w.N;
-      if (written > 0 && !__all_sync(0xffffffffu, mbar_wait(&empty_t, (written - 1) & 1))) {
-        ok = false;
-        break;
-      }
       if (by_bulk(un, n_unit)) {
-        const uint32_t at = smem_u32(ring_o) + part * TC * 256 + (quad * kWarp + lane) * 2;
+        if (written > 0 && !__all_sync(0xffffffffu, mbar_wait(&empty_t, (written - 1) & 1))) {
+          ok = false;
+          break;
+        }
+        const uint32_t at = tile_o + part * TC * 256 + (quad * kWarp + lane) * 2;
 #pragma unroll
         for (int i = 0; i < TC; i += 2) {
           const float lo = 128.f * acc[i / 2].x, hi = 128.f * acc[i / 2].y;
@@ -726,8 +729,7 @@ TcPlan plan_tc(const Q4gParams& p, int sm_count) {
   o.c.nW = 2;
   const int max_s = o.NT == 32 ? Tile<32>::kMaxS : o.NT == 64 ? Tile<64>::kMaxS : o.NT == 128 ? Tile<128>::kMaxS
                                                                                  : Tile<192>::kMaxS;
-  size_t chunks = o.NT >= 128 ? 8 * kChunk * (kWarp + 4) * sizeof(float) : 0;
-  if (o.NT >= 128 && o.c.limbs < 3 && chunks < (size_t)o.NT * 256) chunks = (size_t)o.NT * 256;
+  const size_t chunks = o.NT < 128 ? 0 : kChunkBytes + (o.c.limbs < 3 ? (size_t)o.NT * 256 : 0);
   size_t smem = o.c.nS * stage_s + o.c.nW * stage_w + chunks;
   const int ctas = o.NT <= 64 ? 2 : 1;  // per SM
   while (o.c.nS < max_s && smem + stage_s <= limit) {
@@ -801,11 +803,12 @@ cudaError_t launch_tc_g(const Q4gParams& p, const TcPlan& o, cudaStream_t s) {
 
 // Asked with a kernel that has no tensor memory: of one that has, the runtime
 // counts one CTA to an SM, while two whose columns fit do run together.
-cudaError_t count_clusters() {
-  cudaError_t e = cudaFuncSetAttribute(q4g_planes_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)kTqSmemMax);
-  for (int ctas = 1; ctas <= 2 && e == cudaSuccess; ++ctas)
-    for (int cs = kTqMaxCluster; cs >= 1 && e == cudaSuccess; --cs) {
+void count_clusters() {
+  if (cudaFuncSetAttribute(q4g_planes_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           (int)kTqSmemMax) != cudaSuccess)
+    cudaGetLastError();
+  for (int ctas = 1; ctas <= 2; ++ctas)
+    for (int cs = kTqMaxCluster; cs >= 1; --cs) {
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(cs * 1024);
       cfg.blockDim = dim3(128);
@@ -817,9 +820,13 @@ cudaError_t count_clusters() {
       attr[0].val.clusterDim.z = 1;
       cfg.attrs = attr;
       cfg.numAttrs = 1;
-      e = cudaOccupancyMaxActiveClusters(&g_clusters[ctas][cs], q4g_planes_kernel, &cfg);
+      int n = 0;  // unknown: an even spread
+      if (cudaOccupancyMaxActiveClusters(&n, q4g_planes_kernel, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        n = 0;
+      }
+      g_clusters[ctas][cs] = n;
     }
-  return e;
 }
 
 template <int NT, int G>
@@ -870,7 +877,7 @@ cudaError_t prepare_q4g_tc() {
   if (e == cudaSuccess) e = prepare_tc_g<64>();
   if (e == cudaSuccess) e = prepare_tc_g<128>();
   if (e == cudaSuccess) e = prepare_tc_g<192>();
-  if (e == cudaSuccess && !g_clusters[1][1]) e = count_clusters();  // (every GPU of a node is alike)
+  if (e == cudaSuccess && !g_clusters[1][1]) count_clusters();  // (every GPU of a node is alike)
   return e;
 }
 

@@ -175,3 +175,11 @@ def test_more_tiles_than_sms(ctx, torch_cuda, dtype, pad, accumulate):
 @pytest.mark.parametrize("N,pad", [(3000, 7), (3010, 2)])
 def test_more_gated_tiles_than_sms(ctx, torch_cuda, dtype, N, pad):
     gated_case(ctx, torch_cuda, 700, 256, N, 32, True, pad, "silu", dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_whole_and_cut_tiles_in_turns(ctx, torch_cuda, dtype):
+    """One group of k a tile, so that warps may be a tile apart, and every
+    third tile's columns end inside it."""
+    for seed in range(4):
+        check(torch_cuda, ctx, 40000, 128, 328, 128, True, getattr(torch_cuda, dtype), 7, seed=seed)
