@@ -321,11 +321,11 @@ __global__ void __launch_bounds__(kQgWarps* kWarp, T* NB <= 2 ? 2 : 1)
   uint32_t phase = 0;
   int begun = kb;  // block of the set that this warp's sum starts at
   for (int i = 0; i < n; ++i) {
-    if (!mbar_wait(&full[slot], phase)) {
+    if (!mbar_wait_warp(&full[slot], phase)) {
       if (lane == 0) atomicOr(p.err, kErrWaitTimeout);
       // let the other copies land before the CTA can exit
       for (int j = i + 1; j < min(n, i + p.stages); ++j)
-        mbar_wait(&full[j % p.stages], (j / p.stages) & 1);
+        mbar_wait_warp(&full[j % p.stages], (j / p.stages) & 1);
       ok = false;
       break;
     }

@@ -359,12 +359,9 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
     Ring rs, rd;
     int used = 0;  // accumulators begun
     bool ok = true;
-    auto wait = [&](uint64_t* bar, uint32_t phase) {
-      return __all_sync(0xffffffffu, mbar_wait(bar, phase)) != 0;
-    };
     const int total = stages * n_units;  // (an even number of halves to a tile)
     for (int j = 0; j < total && ok; ++j) {
-      ok = wait(&full_s[rs.slot], rs.phase);
+      ok = mbar_wait_warp(&full_s[rs.slot], rs.phase);
       const uint32_t da = tmem_a + (uint32_t)(rs.slot * HS * 32);
       const uint64_t db = desc_b + (uint32_t)(rs.slot * stage_s / 16);
       tc_fence_after();
@@ -376,7 +373,7 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
           const bool begins = G < 4 || !odd, ends = G < 4 || odd;
           if (begins) {
             if (used >= S_::kD) {
-              ok = ok && wait(&empty_d[rd.slot], rd.phase ^ 1);
+              ok = ok && mbar_wait_warp(&empty_d[rd.slot], rd.phase ^ 1);
               tc_fence_after();
             }
             ++used;
@@ -408,7 +405,7 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
     for (int n = 0; n < n_units; ++n) {
       const Unit t = unit(n);
       if (!by_bulk(t, n)) continue;
-      if (!__all_sync(0xffffffffu, mbar_wait(&full_t, written & 1))) {
+      if (!mbar_wait_warp(&full_t, written & 1)) {
         if (lane == 0) fail();
         break;
       }
@@ -441,13 +438,10 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
     if (HS == 1) rs.next(c.nS, half);
     int n = 0, left = blocks;
     bool live = unit(0).second || quad < 2;  // the tiles exist
-    auto wait = [&](uint64_t* bar, uint32_t phase) {
-      return __all_sync(0xffffffffu, mbar_wait(bar, phase)) != 0;
-    };
     uint4 x[kTiles];
     uint32_t z[kTiles][2];
     auto load = [&]() {  // the tiles of the next block, if it has arrived
-      if (!wait(&full_w[rw.slot], rw.phase)) return false;
+      if (!mbar_wait_warp(&full_w[rw.slot], rw.phase)) return false;
       const uint32_t pc = ring_w_s + rw.slot * stage_w + piece * bb;
 #pragma unroll
       for (int j = 0; j < kTiles; ++j) {
@@ -466,7 +460,7 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
         left = blocks;
         live = unit(++n).second || quad < 2;
       }
-      ok = (HS == 1 ? 2 * kb + half : kb) < c.nS || wait(&empty_s[rs.slot], rs.phase ^ 1);
+      ok = (HS == 1 ? 2 * kb + half : kb) < c.nS || mbar_wait_warp(&empty_s[rs.slot], rs.phase ^ 1);
       if (!ok) break;
       tc_fence_after();
       if (live) {
@@ -541,7 +535,7 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
         for (int g = 0; g < ng; ++g) {
           const float sc = u16_scale((unsigned short)(sb.x & 0xffffu), p.w.bf_scale);
           sb.x = g == 1 ? sb.y : sb.x >> 16;
-          ok = ok && mbar_wait(&full_d[rd.slot], rd.phase);
+          ok = ok && mbar_wait_warp(&full_d[rd.slot], rd.phase);
           if (!ok) break;
           tc_fence_after();
           const uint32_t ta = tmem + ((uint32_t)(quad * kWarp) << 16) + (uint32_t)(rd.slot * (int)kColsD + part * TC);
@@ -572,7 +566,7 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
       const int n0 = un.tile * (p.w2 ? 64 : 128) + quad * (p.w2 ? kWarp / 2 : kWarp);  // first column
       const bool fast = plain && n0 + kWarp <= p.w.N;
       if (by_bulk(un, n_unit)) {
-        if (written > 0 && !__all_sync(0xffffffffu, mbar_wait(&empty_t, (written - 1) & 1))) {
+        if (written > 0 && !mbar_wait_warp(&empty_t, (written - 1) & 1)) {
           ok = false;
           break;
         }
@@ -633,7 +627,7 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
       }
     }
     if (!ok && lane == 0) fail();
-    if (!mbar_wait(&done, 0) && lane == 0) fail();  // no MMA is in flight
+    if (!mbar_wait_warp(&done, 0) && lane == 0) fail();  // no MMA is in flight
     tc_fence_before();
     __syncthreads();
     if (S_::kWalk && c.cs == 1) return;
