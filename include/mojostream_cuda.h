@@ -149,8 +149,10 @@ enum { MS_F32 = 0, MS_BF16 = 1, MS_F16 = 2 };
  * w: [K][N / 2] bytes, low nibble = even column (the layout of
  * ms_q4_weight_create); scales: [K / group][N] IEEE half (MS_F16) or bfloat16
  * (MS_BF16); zeros: [K / group][N] bytes 0..15, or NULL (z = 8 everywhere).
- * Host or device pointers, repacked once (waits for the device; the buffers
- * may be freed afterwards).  K % group == 0, N % 2 == 0; a zero point above
+ * Host or device pointers, repacked once (first waits for all work on the
+ * context's device and on the devices that hold the buffers, so sources that
+ * such work is still writing are read complete, pinned host memory too; the
+ * buffers may be freed afterwards).  K % group == 0, N % 2 == 0; a zero point above
  * 15 is refused (MS_ERR_INVALID_ARG). */
 typedef struct ms_q4g_weight ms_q4g_weight;
 MS_API ms_status ms_q4g_weight_create(ms_ctx *ctx, const uint8_t *w, const void *scales,

@@ -64,6 +64,20 @@ bool on_device(const void* p, int device) {
 
 int type_size(int t) { return t == MS_F32 ? 4 : 2; }
 
+// Work that may still write `src`: everything queued on the device that holds
+// it (null: none), pinned host memory counting for the context's device.
+cudaError_t wait_for_writers(const void* src, int device) {
+  cudaPointerAttributes a;
+  if (!src) return cudaSuccess;
+  if (cudaPointerGetAttributes(&a, src) != cudaSuccess) {
+    cudaGetLastError();
+    return cudaSuccess;
+  }
+  if (a.type != cudaMemoryTypeDevice || a.device == device) return cudaSuccess;  // (waited for already)
+  DeviceGuard other(a.device);
+  return cudaDeviceSynchronize();
+}
+
 // A source matrix on the device: itself, or a copy of host memory.
 struct Staged {
   const void* p = nullptr;
@@ -174,6 +188,11 @@ extern "C" ms_status ms_q4g_weight_create(ms_ctx* c, const uint8_t* w, const voi
   v.block_bytes = q4g_block_bytes(group, v.zeros);
   const size_t bytes = (size_t)q4g_quads(N) * v.nkb * kQgQuad * v.block_bytes;
   const size_t n_groups = (size_t)(K / group) * N;
+  // the sources may still be written by work on other streams, host memory by
+  // copies out of the device: all of it first, then the copies of them
+  OPS_CUDA(c, cudaDeviceSynchronize());
+  for (const void* src : {(const void*)w, scales, (const void*)zeros})
+    OPS_CUDA(c, wait_for_writers(src, dev));
   Staged sw, ss, sz;
   OPS_CUDA(c, sw.take(w, (size_t)K * (N / 2), dev));
   OPS_CUDA(c, ss.take(scales, n_groups * 2, dev));
@@ -181,9 +200,7 @@ extern "C" ms_status ms_q4g_weight_create(ms_ctx* c, const uint8_t* w, const voi
   uint8_t* d = nullptr;
   int* bad = nullptr;
   int h_bad = 0;
-  // the sources may still be written by work on other streams
-  cudaError_t e = cudaDeviceSynchronize();
-  if (e == cudaSuccess) e = cudaMalloc((void**)&d, bytes);
+  cudaError_t e = cudaMalloc((void**)&d, bytes);
   if (e == cudaSuccess) e = cudaMalloc((void**)&bad, sizeof(int));
   if (e == cudaSuccess) e = cudaMemsetAsync(bad, 0, sizeof(int), s);
   if (e == cudaSuccess)

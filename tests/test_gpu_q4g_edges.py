@@ -1,0 +1,49 @@
+"""Group-scaled products and the gated half at the edges of what a caller may do."""
+import numpy as np
+import pytest
+
+from test_gpu_q4g import bound, dense, make_weight, rows
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch_cuda():
+    import torch
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    return torch
+
+
+@pytest.fixture(scope="module")
+def ctx(torch_cuda):
+    from mojostream_b200.runtime import Context
+    c = Context(0)
+    yield c
+    c.close()
+
+
+def test_sources_that_a_stream_still_writes(ctx, torch_cuda):
+    """Pinned host sources filled by copies that wait, on a stream of their
+    own, behind 100 ms of other work: the weight is made of what they bring."""
+    torch = torch_cuda
+    from mojostream_b200.runtime import Q4GroupWeight
+    rng = np.random.default_rng(21)
+    K, N, g = 256, 128, 64
+    q, s, z = make_weight(rng, K, N, g, True)
+    want = [torch.from_numpy(x).cuda() for x in (q, s, z)]
+    host = [torch.zeros(x.shape, dtype=x.dtype).pin_memory() for x in want]
+    a = rows(torch, rng, 3, K, 0, torch.float32)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)
+        for h, x in zip(host, want):
+            h.copy_(x, non_blocking=True)
+    w = Q4GroupWeight(ctx, host[0], host[1], K, N, g, zeros=host[2])
+    c = w.gemm(a, torch.empty((3, N), device="cuda"))
+    ctx.sync(current=True)
+    a64, wd = a.double().cpu().numpy(), dense(q, s, z, g)
+    exact = a64 @ wd
+    assert (np.abs(c.double().cpu().numpy() - exact) <= bound(torch, torch.float32, g, a64, wd, exact)).all()
+    w.close()
