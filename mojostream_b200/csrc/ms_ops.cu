@@ -32,9 +32,11 @@ namespace {
 #define OPS_CUDA(c, call)                                                                       \
   do {                                                                                          \
     const cudaError_t e_ = (call);                                                              \
-    if (e_ != cudaSuccess)                                                                      \
+    if (e_ != cudaSuccess) {                                                                    \
+      cudaGetLastError(); /* reported here: a later launch must not see it again */             \
       OPS_FAIL((c), e_ == cudaErrorMemoryAllocation ? MS_ERR_OOM : MS_ERR_CUDA, "%s: %s", #call, \
                cudaGetErrorString(e_));                                                         \
+    }                                                                                           \
   } while (0)
 
 // The context's device is current inside a call; the caller's comes back after.
@@ -210,7 +212,6 @@ extern "C" ms_status ms_q4g_weight_create(ms_ctx* c, const uint8_t* w, const voi
   cudaFree(bad);
   ms_q4g_weight* h = e == cudaSuccess && !h_bad ? new (std::nothrow) ms_q4g_weight : nullptr;
   if (!h) cudaFree(d);
-  if (e == cudaErrorMemoryAllocation) cudaGetLastError();
   OPS_CUDA(c, e);
   if (h_bad) OPS_FAIL(c, MS_ERR_INVALID_ARG, "ms_q4g_weight_create: a zero point above 15");
   if (!h) OPS_FAIL(c, MS_ERR_OOM, "ms_q4g_weight_create: host memory");

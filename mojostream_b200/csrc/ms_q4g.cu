@@ -574,9 +574,12 @@ cudaError_t launch_q4g_repack(uint8_t* out, const Q4gView& v, const uint8_t* src
                               const uint8_t* zeros, int* bad, cudaStream_t s) {
   const size_t n = (size_t)q4g_quads(v.N) * v.nkb * kQgQuad * (256 + kQgBlockK / v.group * kQgTile);
   const size_t blocks = (n + 255) / 256;
-  q4g_repack_kernel<<<(unsigned)(blocks < 148 * 64 ? blocks : 148 * 64), 256, 0, s>>>(
-      out, v, src, reinterpret_cast<const uint16_t*>(scales), zeros, bad);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(blocks < 148 * 64 ? blocks : 148 * 64));
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  return cudaLaunchKernelEx(&cfg, q4g_repack_kernel, out, v, src,
+                            reinterpret_cast<const uint16_t*>(scales), zeros, bad);
 }
 
 size_t q4g_records_bytes(const Q4gRows& r) {

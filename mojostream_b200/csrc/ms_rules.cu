@@ -384,9 +384,12 @@ template <typename E, int NV>
 cudaError_t launch_t(const RulesParams& p, cudaStream_t s) {
   constexpr int chunk = kRuThreads * NV * (16 / (int)sizeof(E));
   const bool lists = p.n_hist > 0 || p.n_bias > 0;
-  rules_kernel<E, NV><<<dim3((p.V + chunk - 1) / chunk, p.M), kRuThreads,
-                        lists ? rules_smem<E, NV>() : 0, s>>>(p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};  // (the launch's own status, not an older call's)
+  cfg.gridDim = dim3((p.V + chunk - 1) / chunk, p.M);
+  cfg.blockDim = dim3(kRuThreads);
+  cfg.dynamicSmemBytes = lists ? rules_smem<E, NV>() : 0;
+  cfg.stream = s;
+  return cudaLaunchKernelEx(&cfg, rules_kernel<E, NV>, p);
 }
 
 // One kernel, 1024 columns (16-bit types: 2048) per CTA, or two or four times
@@ -403,10 +406,13 @@ cudaError_t launch_e(const RulesParams& p, int sm_count, cudaStream_t s) {
     return launch_t<E, 1>(p, s);
   }
   const bool stream = p.mask || p.logits != p.out;
+  cudaLaunchConfig_t cfg = {};
+  cfg.stream = s;
   if (stream) {
     constexpr int kCols = kRuThreads * 32;
-    rules_stream_kernel<E><<<dim3((p.V + kCols - 1) / kCols, p.M), kRuThreads, 0, s>>>(p);
-    const cudaError_t e = cudaGetLastError();
+    cfg.gridDim = dim3((p.V + kCols - 1) / kCols, p.M);
+    cfg.blockDim = dim3(kRuThreads);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, rules_stream_kernel<E>, p);
     if (e != cudaSuccess) return e;
   }
   if (!lists) return cudaSuccess;
@@ -414,10 +420,8 @@ cudaError_t launch_e(const RulesParams& p, int sm_count, cudaStream_t s) {
   const long long each = ((long long)p.n_hist + p.n_bias) / p.M;
   int sb = 0;
   while (sb < 6 && (((long long)p.M << sb) < sm_count || each >> sb > 1024)) ++sb;
-  cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(1u << sb, p.M, 1);
   cfg.blockDim = dim3(kHsThreads);
-  cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;

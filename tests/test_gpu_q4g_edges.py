@@ -47,3 +47,24 @@ def test_sources_that_a_stream_still_writes(ctx, torch_cuda):
     exact = a64 @ wd
     assert (np.abs(c.double().cpu().numpy() - exact) <= bound(torch, torch.float32, g, a64, wd, exact)).all()
     w.close()
+
+
+def test_a_refused_weight_leaves_no_error_behind(ctx, torch_cuda):
+    """A weight larger than the device is refused, and only that: the calls
+    after it, whose launches also report errors, succeed."""
+    import ctypes
+    torch = torch_cuda
+    from mojostream_b200 import _lib
+    from mojostream_b200.runtime import LogitRules
+    q, s = np.zeros(64, np.uint8), np.zeros(64, np.float16)
+    h = ctypes.c_void_p()
+    for _ in range(2):
+        # 2^39 bytes: no allocation, so nothing of q or s is read
+        status = _lib.lib().ms_q4g_weight_create(ctx.h, q.ctypes.data, s.ctypes.data, 2, None, 1 << 20,
+                                                 1 << 20, 128, ctypes.byref(h))
+        assert _lib.STATUS_NAMES[status] == "MS_ERR_OOM" and not h
+        mask = torch.full((1, 2), 5, dtype=torch.int32, device="cuda")
+        lg = torch.ones((1, 40), device="cuda")
+        ctx.logit_rules(lg, LogitRules(mask=mask))
+        assert torch.isfinite(lg).sum() == 4
+    ctx.sync(current=True)
