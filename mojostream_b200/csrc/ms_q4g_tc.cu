@@ -380,13 +380,15 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
           }
           const uint32_t dt = tmem + (uint32_t)rd.slot * kColsD;
           if (ok && elect_one()) {
-            for (int l = 0; l < c.limbs; ++l)
+            // the smallest limbs first: an MMA cuts its sum off below the
+            // accumulator's last place, which costs least while that is small
+            for (int l = c.limbs - 1; l >= 0; --l)
 #pragma unroll
               for (int k = 0; k < kK16; ++k)
                 umma_bf16_ta(dt, da + h * 32 + (g * kK16 + k) * 8,
                              db + (uint32_t)((h * c.limbs + l) * (kUnitB / 16)) +
                                  (g * kK16 + k) * kStepB,
-                             idesc, k != 0 || l != 0 || !begins);
+                             idesc, k != 0 || l != c.limbs - 1 || !begins);
             if (ends) umma_commit(&full_d[rd.slot]);
             if (h == HS - 1 && g == kSub - 1) umma_commit(&empty_s[rs.slot]);
           }

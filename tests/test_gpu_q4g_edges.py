@@ -68,3 +68,28 @@ def test_a_refused_weight_leaves_no_error_behind(ctx, torch_cuda):
         ctx.logit_rules(lg, LogitRules(mask=mask))
         assert torch.isfinite(lg).sum() == 4
     ctx.sync(current=True)
+
+
+@pytest.mark.parametrize("M", [20, 50, 300])
+@pytest.mark.parametrize("g", [32, 64])
+def test_fp32_sums_of_many_rows_keep_their_last_bits(ctx, torch_cuda, M, g):
+    """The error of all results together (2-norms).  An MMA of 16 k cuts its sum
+    off: half a unit of 2^-23 on average of a partial sum, whose size after
+    the j-th of a group's g / 16 is sqrt(16 j / g) of the group's.  That is if
+    the limbs come smallest first; the smaller limbs after the largest would
+    add 2 g / 16 cuts at full size.  Then K / g sums in fp32, each rounded by
+    2^-24 / sqrt(3) (uniform) of a partial sum of sqrt(j g / K)."""
+    torch = torch_cuda
+    from mojostream_b200.runtime import Q4GroupWeight
+    rng = np.random.default_rng(M + g)
+    K, N = 256, 512
+    q, s, z = make_weight(rng, K, N, g, True)
+    w = Q4GroupWeight(ctx, q, s, K, N, g, zeros=z)
+    a = torch.from_numpy(rng.standard_normal((M, K)).astype(np.float32)).cuda()
+    c = w.gemm(a, torch.empty((M, N), device="cuda")).double().cpu().numpy()
+    exact = a.double().cpu().numpy() @ dense(q, s, z, g)
+    steps, groups = g // 16, K // g
+    cuts = 0.5 * 2.0 ** -23 * sum(((j + 1) / steps) ** 0.5 for j in range(steps))
+    limit = cuts + 2.0 ** -24 / 3 ** 0.5 * ((groups + 1) / 2) ** 0.5
+    assert np.linalg.norm(c - exact) <= limit * np.linalg.norm(exact)
+    w.close()
