@@ -166,15 +166,15 @@ MS_API size_t ms_q4g_weight_bytes(const ms_q4g_weight *w);
  * A and C: device memory of one type (dtype), rows lda >= K and ldc >= N
  * elements apart, aligned to their elements; they must not share memory.
  * M <= 4194304.  Sums are fp32, rounded once to dtype.
- *   Few rows (up to 8 of bfloat16, 16 of fp32 and half): a value is held to
- * 2^-30 (fp32) or 2^-22 of the largest of its group in its row, at least
+ *   Few rows (up to 8 of fp32 and bfloat16, 16 of half): a value is held to
+ * 2^-45 (fp32) or 2^-30 of the largest of its group in its row, at least
  * 2^-120.  More rows: values are used exactly as given.  A group whose sum
  * passes the range of fp32 before its scale is applied (magnitudes near 2^117
  * and up) overflows to infinity or NaN; an infinity or NaN in a row of A makes
  * that row's results infinite or NaN, and no other row's.
  *   The call may use the context's workspace: for each value of A (k rounded
- * up to 128) at most 5 bytes with few rows, rounded up to 8; 2 (bfloat16), 4
- * (half) or 6 (fp32) bytes with more, rounded up to whole tiles of 32 to 192.
+ * up to 128) at most 8 (fp32) or 6 bytes with few rows; 2 (bfloat16), 4 (half)
+ * or 6 (fp32) bytes with more, rounded up to whole tiles of 32 to 192 rows.
  * It grows on the first call of a size, which must not happen inside a stream
  * capture (MS_ERR_STATE), and calls on different streams must not overlap in
  * time, captured and replayed ones included. */

@@ -150,7 +150,6 @@ ms_status run_q4g(ms_ctx* c, const ms_q4g_weight* w, const ms_q4g_weight* w2, in
     OPS_CUDA(c, launch_q4g_tc(p, ms_sm_count_(c), s));
     return MS_OK;
   }
-  if ((M + kQgMaxRows - 1) / kQgMaxRows > 65535) OPS_FAIL(c, MS_ERR_SHAPE, "q4g: M=%d", M);
   if (!q4g_stream_converts(p, ms_sm_count_(c))) {
     void* ws = nullptr;
     const ms_status st = ms_workspace_(c, s, q4g_records_bytes(p.a), &ws);

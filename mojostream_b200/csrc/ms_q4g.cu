@@ -99,66 +99,81 @@ __device__ __forceinline__ void transpose4(const uint32_t* d, uint32_t (&w)[4]) 
 }
 
 // Sixteen lanes: 128 k of a row, 8 consecutive ones (v) per lane hl, into
-// columns c0 .. c0 + 3 of a record with `cols` columns.  Whole warp (two
+// columns c0 .. c0 + D - 1 of a record with `cols` columns.  Whole warp (two
 // rows or blocks at a time); nothing is written where live is false.
 //   A group with a NaN gets the factor NaN; one with infinities holds +-1 at
 // them, 0 elsewhere and the factor infinity, so that infinity * w comes out
 // as it should (NaN for w = 0).
-__device__ __forceinline__ void convert8(const float (&v)[8], int group, int c0, int cols, int hl,
+template <int D>
+__device__ __forceinline__ void convert8(float (&v)[8], int group, int c0, int cols, int hl,
                                          bool live, uint8_t* rec) {
   const int glanes = group / 8, ng = kQgBlockK / group;
   const int c8 = (cols + 7) / 8 * 8;
   uint32_t mx = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) mx = max(mx, __float_as_uint(v[j]) & 0x7fffffffu);
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) {
-    const uint32_t other = __shfl_xor_sync(0xffffffffu, mx, o);
-    if (o < glanes) mx = max(mx, other);
-  }
+  for (int o = 1; o < glanes; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   // exponent of the largest value; groups below 2^-90 share its scale
   constexpr int top = 29;
   const int e = max((int)(mx >> 23) - 127, -90);
   const bool finite = mx < 0x7f800000u;
-  const float up = finite ? pow2(top - e) : 0.f;
-  uint32_t d[8];  // the digits of q: q + 0x80808080 with every byte's top bit flipped
+  constexpr int P = D > 4 ? 2 : 1;
+  uint32_t w[P][2][4];  // digit words of the lane's 8 k
+  int sum[D / 2];       // digit sums of the lane's, then the group's k
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    int q = __float2int_rn(v[j] * up);
-    if (!finite) q = isinf(v[j]) ? (v[j] > 0.f ? 1 : -1) : 0;
-    d[j] = ((uint32_t)q + 0x80808080u) ^ 0x80808080u;
-  }
-  uint32_t w0[4], w1[4];
-  transpose4(d, w0);
-  transpose4(d + 4, w1);
-  // digit sums of the lane's 8 k, two digits to a word (|sum| <= 2^14)
-  int s[4], s02, s13;
+  for (int p = 0; p < P; ++p) {
+    const int x = min(top - e + 15 * p, 126);
+    const float up = finite ? pow2(x) : 0.f, down = pow2(-x);
+    uint32_t d[8];  // the digits of q: q + 0x80808080 with every byte's top bit flipped
 #pragma unroll
-  for (int l = 0; l < 4; ++l) s[l] = __dp4a((int)w1[l], 0x01010101, __dp4a((int)w0[l], 0x01010101, 0));
-  s02 = s[0] + s[2] * 65536;
-  s13 = s[1] + s[3] * 65536;
+    for (int j = 0; j < 8; ++j) {
+      int q = __float2int_rn(v[j] * up);
+      if (!finite) q = p == 0 && isinf(v[j]) ? (v[j] > 0.f ? 1 : -1) : 0;
+      d[j] = ((uint32_t)q + 0x80808080u) ^ 0x80808080u;
+      // what is left, exactly: q has no more bits than v where it is not 0
+      if (p + 1 < P) v[j] = fmaf(-(float)q, down, v[j]);
+    }
+    transpose4(d, w[p][0]);
+    transpose4(d + 4, w[p][1]);
+    // two digits of the first four, l and l + 2, to a word (|sum| <= 2^14); so
+    // the last two
+    int s[4];
 #pragma unroll
-  for (int o = 1; o < 16; o <<= 1) {
-    const int x = __shfl_xor_sync(0xffffffffu, s02, o), y = __shfl_xor_sync(0xffffffffu, s13, o);
-    if (o < glanes) {
-      s02 += x;
-      s13 += y;
+    for (int l = 0; l < 4; ++l)
+      s[l] = __dp4a((int)w[p][1][l], 0x01010101, __dp4a((int)w[p][0][l], 0x01010101, 0));
+    if (p == 0) {
+      sum[0] = s[0] + s[2] * 65536;
+      sum[1] = s[1] + s[3] * 65536;
+    } else {
+      sum[D / 2 - 1] = s[0] + s[1] * 65536;
     }
   }
+  for (int o = 1; o < glanes; o <<= 1)
+#pragma unroll
+    for (int i = 0; i < D / 2; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
   if (!live) return;
   // 4 lanes per 32-k step, two steps to a half
   uint8_t* dst = rec + ((hl >> 3) * cols + c0) * 64 + (hl & 3) * 16 + ((hl >> 2) & 1) * 8;
 #pragma unroll
-  for (int l = 0; l < 4; ++l) *reinterpret_cast<uint2*>(dst + l * 64) = make_uint2(w0[l], w1[l]);
+  for (int l = 0; l < D; ++l)
+    *reinterpret_cast<uint2*>(dst + l * 64) = make_uint2(w[l / 4][0][l & 3], w[l / 4][1][l & 3]);
   if (hl % glanes == 0) {
     const int at = hl / glanes * c8 + c0;
     float* f = reinterpret_cast<float*>(rec + (size_t)cols * 128);
-    const float f0 = finite ? pow2(e - top) : mx > 0x7f800000u ? __uint_as_float(0x7fc00000u) : INFINITY;
+    int2* n = reinterpret_cast<int2*>(reinterpret_cast<int*>(f + ng * c8 / 2) + at);
+    const float f0 = finite ? pow2(e - top)
+                            : mx > 0x7f800000u ? __uint_as_float(0x7fc00000u) : INFINITY;
     // (an infinity sits in the first digit alone)
-    *reinterpret_cast<float2*>(f + at / 2) = make_float2(f0, finite ? f0 * 65536.f : 0.f);
-    const int lo02 = (int)(short)s02, lo13 = (int)(short)s13;
-    *reinterpret_cast<int4*>(reinterpret_cast<int*>(f + ng * c8 / 2) + at) =
-        make_int4(lo02, lo13, (s02 - lo02) >> 16, (s13 - lo13) >> 16);
+    f[at / 2] = f0;
+    f[at / 2 + 1] = finite ? f0 * 65536.f : 0.f;
+    const int lo02 = (int)(short)sum[0], lo13 = (int)(short)sum[1];
+    n[0] = make_int2(lo02, lo13);
+    n[1] = make_int2((sum[0] - lo02) >> 16, (sum[1] - lo13) >> 16);
+    if (P == 2) {
+      f[at / 2 + 2] = finite ? pow2(-min(top - e + 15, 126)) : 0.f;
+      const int lo = (int)(short)sum[D / 2 - 1];
+      n[2] = make_int2(lo, (sum[D / 2 - 1] - lo) >> 16);
+    }
   }
 }
 
@@ -167,13 +182,17 @@ __global__ void __launch_bounds__(256) q4g_rows_kernel(const Q4gRows a) {
   pdl_wait();     // the rows are an earlier kernel's output, and the records
   pdl_trigger();  // may still be read by the product before this one
   const int kb = blockIdx.x * 16 + (threadIdx.x >> 4), hl = threadIdx.x & 15;
+  const int digits = qg_digits(a.type), per = qg_block_rows(a.type, a.M);
   for (int m = blockIdx.y; m < a.M; m += gridDim.y) {
-    const int rb = m / kQgMaxRows, rows = min(kQgMaxRows, a.M - rb * kQgMaxRows);
+    const int rb = m / per, cols = min(per, a.M - rb * per) * digits;
     float v[8];
     load8(a, m, kb * kQgBlockK + 8 * hl, v);
-    uint8_t* rec = a.records + rb * (size_t)a.nkb * qg_record_bytes(kQgMaxRows, a.group) +
-                   (size_t)kb * qg_record_bytes(rows, a.group);
-    convert8(v, a.group, m % kQgMaxRows * kQgDigits, rows * kQgDigits, hl, kb < a.nkb, rec);
+    uint8_t* rec = a.records + rb * (size_t)a.nkb * qg_record_bytes(per * digits, a.group) +
+                   (size_t)kb * qg_record_bytes(cols, a.group);
+    if (digits == 6)
+      convert8<6>(v, a.group, m % per * 6, cols, hl, kb < a.nkb, rec);
+    else
+      convert8<4>(v, a.group, m % per * 4, cols, hl, kb < a.nkb, rec);
   }
 }
 
@@ -210,8 +229,9 @@ struct Split {
   }
 };
 
-// NB: 8-column blocks of digits (2 rows each); G: 32-k steps per group (1, 2, 4).
-template <int T, int NB, int G>
+// NB: 8-column blocks of digits (two rows of four digits each, or 4/3 rows of
+// six); G: 32-k steps per group (1, 2, 4); wide: fp32 rows.
+template <int T, int NB, int G, bool wide>
 __global__ void __launch_bounds__(kQgWarps* kWarp, T* NB <= 2 ? 2 : 1)
     q4g_stream_kernel(const Q4gParams p) {
   extern __shared__ __align__(128) uint8_t dsm[];
@@ -225,8 +245,11 @@ __global__ void __launch_bounds__(kQgWarps* kWarp, T* NB <= 2 ? 2 : 1)
   const int cols = per * kQgTile;    // result columns of a set
   const int nkb = p.w.nkb, bb = p.w.block_bytes;
   constexpr int ng = 4 / G;
-  const int row0 = blockIdx.y * kQgMaxRows, rows = min(kQgMaxRows, p.a.M - row0);
-  const int C = rows * kQgDigits, rc8 = (C + 7) / 8 * 8;
+  constexpr int digits = wide ? 6 : 4;
+  constexpr int kRows = wide ? NB * 8 / 6 : NB;  // loops over rows of six digits, or blocks
+  const int row_block = qg_block_rows(p.a.type, p.a.M);
+  const int row0 = blockIdx.y * row_block, rows = min(row_block, p.a.M - row0);
+  const int C = rows * digits, rc8 = (C + 7) / 8 * 8;
   const int rec = C * 128 + ng * rc8 * 6;
   const bool own_a = p.a.records == nullptr;
   const int stage_bytes = T * bb + (own_a ? 0 : rec);
@@ -260,7 +283,7 @@ __global__ void __launch_bounds__(kQgWarps* kWarp, T* NB <= 2 ? 2 : 1)
   seek();
   const uint8_t* a_src =
       own_a ? nullptr
-            : p.a.records + (size_t)blockIdx.y * nkb * qg_record_bytes(kQgMaxRows, p.w.group);
+            : p.a.records + (size_t)blockIdx.y * nkb * qg_record_bytes(row_block * digits, p.w.group);
   auto issue_w = [&](int slot) {
     uint8_t* st = ring + slot * stage_bytes;
     mbar_expect_tx(&full[slot], stage_bytes);
@@ -295,7 +318,7 @@ __global__ void __launch_bounds__(kQgWarps* kWarp, T* NB <= 2 ? 2 : 1)
     for (; __any_sync(0xffffffffu, it < items); it += 2 * kQgWarps) {
       const int nt = it + 2 * kQgWarps;
       load8(p.a, row0 + nt / nkb, nt < items ? nt % nkb * kQgBlockK + 8 * hl : p.a.K, nx);
-      convert8(v, p.w.group, it / nkb * kQgDigits, C, hl, it < items, dsm + (size_t)(it % nkb) * rec);
+      convert8<digits>(v, p.w.group, it / nkb * digits, C, hl, it < items, dsm + (size_t)(it % nkb) * rec);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = nx[j];
     }
@@ -309,11 +332,24 @@ __global__ void __launch_bounds__(kQgWarps* kWarp, T* NB <= 2 ? 2 : 1)
   for (int i = 0; i < T; ++i)
 #pragma unroll
     for (int b = 0; b < NB; ++b) acc[i][b][0] = acc[i][b][1] = 0.f;
-  // a row's digits are with lanes t = 0, 1 (row 0 of a column block) or 2, 3 (row 1)
-  auto row_sums = [&](int j, int b, float& lo, float& hi) {
-    lo = acc[j][b][0] + __shfl_xor_sync(0xffffffffu, acc[j][b][0], 1);
-    hi = acc[j][b][1] + __shfl_xor_sync(0xffffffffu, acc[j][b][1], 1);
+  // The sums of tile j: of row i of six digits, in pairs 3 i .. 3 i + 2 (lane t
+  // of column block b has pair 4 b + t), or of row 2 i (lanes t = 0, 1) or
+  // 2 i + 1 (t = 2, 3).  `mine`: this lane has a row of its own, m.
+  auto row_sums = [&](int j, int i, float& lo, float& hi) {
+    if constexpr (wide) {
+      lo = hi = 0.f;
+#pragma unroll
+      for (int q = 3 * i; q < 3 * i + 3; ++q) {
+        lo += __shfl_sync(0xffffffffu, acc[j][q >> 2][0], (lane & 28) | (q & 3));
+        hi += __shfl_sync(0xffffffffu, acc[j][q >> 2][1], (lane & 28) | (q & 3));
+      }
+    } else {
+      lo = acc[j][i][0] + __shfl_xor_sync(0xffffffffu, acc[j][i][0], 1);
+      hi = acc[j][i][1] + __shfl_xor_sync(0xffffffffu, acc[j][i][1], 1);
+    }
   };
+  auto row_of = [&](int i) { return wide ? i : 2 * i + (t >> 1); };
+  auto mine = [&](int i) { return wide ? t == (i & 3) && i < rows : !(t & 1) && 2 * i + (t >> 1) < rows; };
 
   const uint32_t dsm_s = smem_u32(dsm), ring_s = smem_u32(ring);
   bool ok = true;
@@ -426,15 +462,15 @@ __global__ void __launch_bounds__(kQgWarps* kWarp, T* NB <= 2 ? 2 : 1)
 #pragma unroll
         for (int j = 0; j < T; ++j)
 #pragma unroll
-          for (int b = 0; b < NB; ++b) {
+          for (int i2 = 0; i2 < kRows; ++i2) {
             float lo, hi, ulo = 0.f, uhi = 0.f;
             if (p.w2 && j >= T / 2) break;
-            row_sums(j, b, lo, hi);
-            if (p.w2) row_sums((j + T / 2) % T, b, ulo, uhi);
-            const int m = 2 * b + (t >> 1);
-            if (!(t & 1) && m < rows) {
-              finish(p, row0 + m, set * cols + j * kQgTile + r, lo, ulo);
-              finish(p, row0 + m, set * cols + j * kQgTile + r + 8, hi, uhi);
+            row_sums(j, i2, lo, hi);
+            if (p.w2) row_sums((j + T / 2) % T, i2, ulo, uhi);
+            if (mine(i2)) {
+              const int m = row0 + row_of(i2);
+              finish(p, m, set * cols + j * kQgTile + r, lo, ulo);
+              finish(p, m, set * cols + j * kQgTile + r + 8, hi, uhi);
             }
           }
       } else {
@@ -442,13 +478,13 @@ __global__ void __launch_bounds__(kQgWarps* kWarp, T* NB <= 2 ? 2 : 1)
 #pragma unroll
         for (int j = 0; j < T; ++j)
 #pragma unroll
-          for (int b = 0; b < NB; ++b) {
+          for (int i2 = 0; i2 < kRows; ++i2) {
             float lo, hi;
-            row_sums(j, b, lo, hi);
-            const int m = 2 * b + (t >> 1);
-            if (!(t & 1) && m < rows) {
-              d[m * kCols + j * kQgTile + r] = lo;
-              d[m * kCols + j * kQgTile + r + 8] = hi;
+            row_sums(j, i2, lo, hi);
+            if (mine(i2)) {
+              float* at = d + row_of(i2) * kCols + j * kQgTile + r;
+              at[0] = lo;
+              at[8] = hi;
             }
           }
       }
@@ -492,24 +528,25 @@ struct StreamPlan {
 
 StreamPlan plan_stream(const Q4gParams& p, int sm_count) {
   StreamPlan o{};
-  const int rows = p.a.M < kQgMaxRows ? p.a.M : kQgMaxRows;
-  const int row_blocks = (p.a.M + kQgMaxRows - 1) / kQgMaxRows;
-  o.NB = (rows + 1) / 2;
+  const int digits = qg_digits(p.a.type), per = qg_block_rows(p.a.type, p.a.M);  // rows of a block
+  const int row_blocks = (p.a.M + per - 1) / per;
+  o.NB = (per * digits + 7) / 8;
   // four tiles to a set share a block's loads and loop (one row, K 2560, N
   // 20480: 7.6 us, with two 8.6 us) where the GPU still gets a set per SM;
   // fewer columns fill it better with two (N 2560: 4.5 us, with four 4.6 us).
-  // From five rows on four tiles' sums do not fit the registers.
+  // From five rows (three of fp32) on four tiles' sums do not fit the registers.
   const int quads = q4g_quads(p.w.N) * (p.w2 ? 2 : 1);
   o.T = o.NB <= 2 && quads >= sm_count ? 4 : 2;
   o.sets = quads * kQgQuad / o.T;
-  // rows x blocks that 16 warps convert in two rounds (one or two rows: three);
-  // more come converted, a launch more (one row, K 10240, N 5120 fp32: 14.4 us,
-  // and 17.3 us; four rows, K 2560: 8.1 and 7.3 us)
-  const size_t rec = (size_t)qg_record_bytes(rows, p.w.group);
+  // rows x blocks that 16 warps convert in two rounds (one or two rows: three,
+  // more fp32 rows: one); more come converted, a launch more (one row, K 10240, N
+  // 5120 bfloat16: 14.4 us, and 17.3 us; four rows, K 2560: 8.1 and 7.3 us; fp32,
+  // four rows, K 1280: 6.0 and 5.5 us)
+  const size_t rec = (size_t)qg_record_bytes(per * digits, p.w.group);
   const size_t a_all = p.w.nkb * rec;
-  o.a_smem = row_blocks == 1 && rows * p.w.nkb <= (rows <= 2 ? 6 : 4) * kQgWarps && a_all <= 64 * 1024 ? a_all : 0;
+  o.a_smem = row_blocks == 1 && per * p.w.nkb <= (per <= 2 ? 6 : digits == 6 ? 2 : 4) * kQgWarps && a_all <= 64 * 1024 ? a_all : 0;
   const size_t stage = (size_t)o.T * p.w.block_bytes + (o.a_smem ? 0 : rec);
-  const size_t fixed = o.a_smem + (size_t)kQgWarps * 2 * rows * o.T * kQgTile * sizeof(float);
+  const size_t fixed = o.a_smem + (size_t)kQgWarps * 2 * per * o.T * kQgTile * sizeof(float);
   // small sets run two CTAs to an SM (64 registers)
   const bool two = o.T * o.NB <= 2 && fixed + 2 * stage * kQgWarps <= kQgSmemMax / 2;
   o.ctas = sm_count * (two ? 2 : 1);
@@ -524,7 +561,7 @@ StreamPlan plan_stream(const Q4gParams& p, int sm_count) {
   return o;
 }
 
-template <int T, int NB, int G>
+template <int T, int NB, int G, bool wide>
 cudaError_t launch_stream_t(const Q4gParams& p0, const StreamPlan& o, cudaStream_t s) {
   Q4gParams p = p0;
   p.stages = o.stages;
@@ -534,7 +571,8 @@ cudaError_t launch_stream_t(const Q4gParams& p0, const StreamPlan& o, cudaStream
   if (o.stages < 1 || o.smem > kQgSmemMax || !p.a.records != (o.a_smem > 0))
     return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(o.ctas, (p.a.M + kQgMaxRows - 1) / kQgMaxRows, 1);
+  const int per = qg_block_rows(p.a.type, p.a.M);
+  cfg.gridDim = dim3(o.ctas, (p.a.M + per - 1) / per, 1);
   cfg.blockDim = dim3(kQgWarps * kWarp);
   cfg.dynamicSmemBytes = o.smem;
   cfg.stream = s;
@@ -543,21 +581,37 @@ cudaError_t launch_stream_t(const Q4gParams& p0, const StreamPlan& o, cudaStream
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, q4g_stream_kernel<T, NB, G>, p);
+  return cudaLaunchKernelEx(&cfg, q4g_stream_kernel<T, NB, G, wide>, p);
 }
 
-template <int T, int NB>
+template <int T, int NB, bool wide>
 cudaError_t launch_stream_g(const Q4gParams& p, const StreamPlan& o, cudaStream_t s) {
   switch (p.w.group) {
-    case 32: return launch_stream_t<T, NB, 1>(p, o, s);
-    case 64: return launch_stream_t<T, NB, 2>(p, o, s);
-    default: return launch_stream_t<T, NB, 4>(p, o, s);
+    case 32: return launch_stream_t<T, NB, 1, wide>(p, o, s);
+    case 64: return launch_stream_t<T, NB, 2, wide>(p, o, s);
+    default: return launch_stream_t<T, NB, 4, wide>(p, o, s);
   }
+}
+
+template <bool wide>
+cudaError_t launch_stream_w(const Q4gParams& p, const StreamPlan& o, cudaStream_t s) {
+  switch (o.T * 8 + o.NB) {  // the plan's own shape, or nothing
+    case 2 * 8 + 1: return launch_stream_g<2, 1, wide>(p, o, s);
+    case 4 * 8 + 1: return launch_stream_g<4, 1, wide>(p, o, s);
+    case 4 * 8 + 2: return launch_stream_g<4, 2, wide>(p, o, s);
+    case 2 * 8 + 2: return launch_stream_g<2, 2, wide>(p, o, s);
+    case 2 * 8 + 3: return launch_stream_g<2, 3, wide>(p, o, s);
+    case 2 * 8 + 4: return launch_stream_g<2, 4, wide>(p, o, s);
+  }
+  return cudaErrorInvalidValue;
 }
 
 template <int T, int NB, int G>
 cudaError_t prepare_t() {
-  return cudaFuncSetAttribute(q4g_stream_kernel<T, NB, G>,
+  const cudaError_t e = cudaFuncSetAttribute(
+      q4g_stream_kernel<T, NB, G, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kQgSmemMax);
+  if (e != cudaSuccess) return e;
+  return cudaFuncSetAttribute(q4g_stream_kernel<T, NB, G, true>,
                               cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kQgSmemMax);
 }
 template <int T, int NB>
@@ -583,8 +637,9 @@ cudaError_t launch_q4g_repack(uint8_t* out, const Q4gView& v, const uint8_t* src
 }
 
 size_t q4g_records_bytes(const Q4gRows& r) {
-  return (size_t)((r.M + kQgMaxRows - 1) / kQgMaxRows) * r.nkb *
-         qg_record_bytes(kQgMaxRows, r.group);
+  const int per = qg_block_rows(r.type, r.M);
+  return (size_t)((r.M + per - 1) / per) * r.nkb *
+         qg_record_bytes(per * qg_digits(r.type), r.group);
 }
 
 cudaError_t launch_q4g_rows(const Q4gRows& r, cudaStream_t s) {
@@ -606,15 +661,7 @@ bool q4g_stream_converts(const Q4gParams& p, int sm_count) {
 
 cudaError_t launch_q4g_stream(const Q4gParams& p, int sm_count, cudaStream_t s) {
   const StreamPlan o = plan_stream(p, sm_count);
-  switch (o.T * 8 + o.NB) {  // the plan's own shape, or nothing
-    case 2 * 8 + 1: return launch_stream_g<2, 1>(p, o, s);
-    case 4 * 8 + 1: return launch_stream_g<4, 1>(p, o, s);
-    case 4 * 8 + 2: return launch_stream_g<4, 2>(p, o, s);
-    case 2 * 8 + 2: return launch_stream_g<2, 2>(p, o, s);
-    case 2 * 8 + 3: return launch_stream_g<2, 3>(p, o, s);
-    case 2 * 8 + 4: return launch_stream_g<2, 4>(p, o, s);
-  }
-  return cudaErrorInvalidValue;
+  return p.a.type == kQgF32 ? launch_stream_w<true>(p, o, s) : launch_stream_w<false>(p, o, s);
 }
 
 cudaError_t prepare_q4g() {

@@ -51,20 +51,33 @@ __host__ __device__ inline int q4g_quads(int N) { return (N + 63) / 64; }
 // Element types of activations and results (MS_F32, MS_BF16, MS_F16).
 enum QgType : int { kQgF32 = 0, kQgBf16 = 1, kQgF16 = 2 };
 
-// Decode rows (streaming kernel): activations as four signed 8-bit digits.
-// For a row and a group of k with 2^e <= max |a| < 2^(e + 1),
-// q = rint(a 2^(29 - e)) = sum_l d_l 256^l: a value within 2^6 (fp32) or 2^21
-// (bfloat16) of its group's largest is held exactly, any other to 2^-30 of the
-// largest.  A digit of a row is a column of the MMA: C = 4 rows, padded to a
+// Decode rows (streaming kernel): activations as signed 8-bit digits.  For a row
+// and a group of k with 2^e <= max |a| < 2^(e + 1),
+// q = rint(a 2^(29 - e)) = sum_l d_l 256^l, l = 0..3: a value within 2^6 (fp32),
+// 2^19 (half) or 2^22 (bfloat16) of its group's largest is held exactly, any
+// other to 2^-30 of the largest.  That is enough for results of 16 bits.  fp32
+// rows have two more digits, rint(r 2^(44 - e)) of what q leaves of a value, so a
+// value within 2^21 of the largest is exact and any other held to 2^-45 of it: a
+// large channel whose weights are q = z adds nothing to a result, and must not
+// take bits from the channels that do (one of 1e4 beside values around 1 cost
+// 3e-6 of the result with four digits, where fp32 itself costs 3e-7).
+//   A digit of a row is a column of the MMA: C = rows x digits <= 32, padded to a
 // multiple of 8.  Record of a 128-k block:
 //   2 x [C] x 64 bytes   the 64-k halves of each column, in fragment order
-//   [128 / g][C8 / 2] float  factors 2^(e - 29), 2^(e - 13) of a row's lower
-//                            and upper two digits
+//   [128 / g][C8 / 2] float  factors of the pairs of digits: 2^(e - 29),
+//                            2^(e - 13), fp32: 2^(e - 44)
 //   [128 / g][C8] int        sums of the group's digits
-constexpr int kQgMaxRows = 8;
-constexpr int kQgDigits = 4;
-__host__ __device__ inline int qg_record_bytes(int rows, int group) {
-  return rows * kQgDigits * 128 + (kQgBlockK / group) * ((rows + 1) / 2 * 8) * 6;
+constexpr int kQgCols = 32;
+__host__ __device__ inline int qg_digits(int type) { return type == kQgF32 ? 6 : 4; }
+// Rows of a block (a launch's grid y, a run of records): at most 8, of fp32 5,
+// and there about the same in every block.
+__host__ __device__ inline int qg_block_rows(int type, int M) {
+  if (type != kQgF32) return M < 8 ? M : 8;
+  const int blocks = (M + 4) / 5;
+  return (M + blocks - 1) / blocks;
+}
+__host__ __device__ inline int qg_record_bytes(int cols, int group) {
+  return cols * 128 + (kQgBlockK / group) * ((cols + 7) / 8 * 8) * 6;
 }
 
 struct Q4gRows {
@@ -72,7 +85,7 @@ struct Q4gRows {
   long long lda;
   int type, M, K, nkb, group;
   int vec;           // rows start on 16-byte boundaries
-  uint8_t* records;  // [row block of 8][128-k block]; many rows: limb planes
+  uint8_t* records;  // [row block][128-k block]; many rows: limb planes
 };
 
 struct Q4gParams {
@@ -91,21 +104,22 @@ struct Q4gParams {
 
 cudaError_t launch_q4g_repack(uint8_t* out, const Q4gView& v, const uint8_t* src, const void* scales,
                               const uint8_t* zeros, int* bad, cudaStream_t s);
-// Rows to records, blocks of kQgMaxRows rows.
+// Rows to records, in blocks of qg_block_rows.
 cudaError_t launch_q4g_rows(const Q4gRows& r, cudaStream_t s);
 size_t q4g_records_bytes(const Q4gRows& r);
-// Any number of rows, kQgMaxRows at a time.  q4g_stream_converts: the launch
-// needs no records.
+// Fewer rows than q4g_tc_rows, qg_block_rows at a time.  q4g_stream_converts:
+// the launch needs no records.
 bool q4g_stream_converts(const Q4gParams& p, int sm_count);
 cudaError_t launch_q4g_stream(const Q4gParams& p, int sm_count, cudaStream_t s);
 cudaError_t prepare_q4g();
 // Many rows on tcgen05 (ms_q4g_tc.cu): two launches; p.a.records is workspace
 // of q4g_planes_bytes.
 // From how many rows on: 9 bfloat16 rows (K 13824, N 5120: 27 us, two rounds of
-// the streaming kernel 37 us; 8 rows 27 and 27 us), 17 rows that take two or
-// three limbs (K 2560, N 20480 half: 16 rows 29 and 27 us, 20 rows 29 and 35 us;
-// K 5120, N 13824 fp32: 34 and 36, 34 and 50 us).
-inline int q4g_tc_rows(int type) { return type == kQgBf16 ? 9 : 17; }
+// the streaming kernel 37 us; 8 rows 27 and 27 us), 17 half rows, of two limbs
+// (K 2560, N 20480: 16 rows 29 and 27 us, 20 rows 29 and 35 us), 9 fp32 rows, of
+// three limbs here and six digits there (K 5120, N 13824: 8 rows 32 and 31 us,
+// 10 rows 32 and 38 us; K 10240, N 2560: 8 rows 18 and 21 us, 5 rows 18 and 14).
+inline int q4g_tc_rows(int type) { return type == kQgF16 ? 17 : 9; }
 size_t q4g_planes_bytes(const Q4gParams& p, int sm_count);
 cudaError_t launch_q4g_tc(const Q4gParams& p, int sm_count, cudaStream_t s);
 cudaError_t prepare_q4g_tc();

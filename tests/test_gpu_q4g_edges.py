@@ -93,3 +93,36 @@ def test_fp32_sums_of_many_rows_keep_their_last_bits(ctx, torch_cuda, M, g):
     limit = cuts + 2.0 ** -24 / 3 ** 0.5 * ((groups + 1) / 2) ** 0.5
     assert np.linalg.norm(c - exact) <= limit * np.linalg.norm(exact)
     w.close()
+
+
+@pytest.mark.parametrize("M", [1, 2, 3, 5, 8, 9, 40])
+@pytest.mark.parametrize("large", [1e4, 1e6])
+def test_a_large_channel_of_weights_zero_takes_no_bits(ctx, torch_cuda, M, large):
+    """Two channels of every group are `large` and meet weights that are 0, the
+    rest are around 1: the error is that of fp32 sums of the rest, however many
+    rows the call has.  With 2-norms and independent roundings (uniform,
+    2^-24 / sqrt(3) each): a group's sum is converted, scaled and added (three),
+    partial sums grow as sqrt(groups); of more rows the MMAs cut off half a
+    unit of 2^-23 four times a group at most.  A value is held to 2^-45 of the
+    largest: less than 2^-25 of 1."""
+    torch = torch_cuda
+    from mojostream_b200.runtime import Q4GroupWeight
+    rng = np.random.default_rng(M)
+    K, N, g = 256, 512, 64
+    q, s, z = make_weight(rng, K, N, g, True)
+    big = np.arange(K).reshape(-1, g)[:, [5, 40]].ravel()
+    zz = np.repeat(z, g, 0)[big]
+    q[big] = zz[:, 0::2] | (zz[:, 1::2] << 4)
+    x = rng.standard_normal((M, K)).astype(np.float32)
+    x[:, big] *= large
+    a = torch.from_numpy(x).cuda()
+    w = Q4GroupWeight(ctx, q, s, K, N, g, zeros=z)
+    c = w.gemm(a, torch.empty((M, N), device="cuda")).double().cpu().numpy()
+    wd = dense(q, s, z, g)
+    assert not wd[big].any()
+    exact = x.astype(np.float64) @ wd
+    limit = 2.0 ** -24 / 3 ** 0.5 * (3 ** 0.5 + ((K // g + 1) / 2) ** 0.5) + 2.0 ** -25
+    if M > 8:
+        limit += 0.5 * 2.0 ** -23 * 4
+    assert np.linalg.norm(c - exact) <= limit * np.linalg.norm(exact)
+    w.close()
