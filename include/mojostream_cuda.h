@@ -171,7 +171,7 @@ MS_API size_t ms_q4g_weight_bytes(const ms_q4g_weight *w);
  * 2^-120.  More rows: values are used exactly as given.  A group whose sum
  * passes the range of fp32 before its scale is applied (magnitudes near 2^117
  * and up) overflows to infinity or NaN; an infinity or NaN in a row of A makes
- * that row's results infinite or NaN, and no other row's.
+ * that row's results infinite or NaN as the formula does, and no other row's.
  *   The call may use the context's workspace: for each value of A (k rounded
  * up to 128) at most 8 (fp32) or 6 bytes with few rows; 2 (bfloat16), 4 (half)
  * or 6 (fp32) bytes with more, rounded up to whole tiles of 32 to 192 rows.

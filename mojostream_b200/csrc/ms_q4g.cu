@@ -103,7 +103,8 @@ __device__ __forceinline__ void transpose4(const uint32_t* d, uint32_t (&w)[4]) 
 // rows or blocks at a time); nothing is written where live is false.
 //   A group with a NaN gets the factor NaN; one with infinities holds +-1 at
 // them, 0 elsewhere and the factor infinity, so that infinity * w comes out
-// as it should (NaN for w = 0).
+// as it should (NaN for w = 0).  Of several infinities only the sum of their
+// weights is seen so: undefined_sum corrects the results that it gets wrong.
 template <int D>
 __device__ __forceinline__ void convert8(float (&v)[8], int group, int c0, int cols, int hl,
                                          bool live, uint8_t* rec) {
@@ -194,6 +195,31 @@ __global__ void __launch_bounds__(256) q4g_rows_kernel(const Q4gRows a) {
     else
       convert8<4>(v, a.group, m % per * 4, cols, hl, kb < a.nkb, rec);
   }
+}
+
+// Whether the sum of row m and column n is NaN by its infinities: one of them
+// meets a weight of 0, or two products are infinities of opposite sign.
+__device__ __forceinline__ bool undefined_sum(const Q4gParams& p, const uint8_t* w, int m, int n) {
+  const int tile = n / kQgTile, c = n % kQgTile, bb = p.w.block_bytes;
+  const uint8_t* piece = w + ((size_t)(tile / kQgQuad) * p.w.nkb * kQgQuad + tile % kQgQuad) * bb;
+  bool pos = false, neg = false;
+#pragma unroll 1
+  for (int k = 0; k < p.w.K; ++k) {
+    const float x = load_out(p.a.a, (size_t)m * p.a.lda + k, p.a.type);
+    if (!isinf(x)) continue;
+    const uint8_t* b = piece + (size_t)(k / kQgBlockK) * kQgQuad * bb;
+    const int kk = k % 64, g = k % kQgBlockK / p.w.group;
+    const int word = (k % kQgBlockK / 64 * 32 + (c & 7) * 4 + kk % 32 / 8) * 4 + kk / 32 * 2 + kk % 8 / 4;
+    const int bit = (kk & 2) * 4 + (kk & 1) * 16 + (c >> 3) * 4, at = (g * 8 + (c & 7)) * 2 + (c >> 3);
+    const int q = (reinterpret_cast<const uint32_t*>(b)[word] >> bit) & 15u;
+    const int z = p.w.zeros ? b[kQgNibbles + kQgBlockK / p.w.group * 32 + at] : 8;
+    const float y = (float)(q - z) *
+                    u16_scale(reinterpret_cast<const uint16_t*>(b + kQgNibbles)[at], p.w.bf_scale);
+    if (!(y > 0.f || y < 0.f)) return true;
+    pos |= (x > 0.f) == (y > 0.f);
+    neg |= (x > 0.f) != (y > 0.f);
+  }
+  return pos && neg;
 }
 
 // ----------------------------------------------------- streaming kernel --
@@ -353,6 +379,7 @@ __global__ void __launch_bounds__(kQgWarps* kWarp, T* NB <= 2 ? 2 : 1)
 
   const uint32_t dsm_s = smem_u32(dsm), ring_s = smem_u32(ring);
   bool ok = true;
+  bool odd = false;  // an infinity or a NaN among the sums
   int slot = 0;
   uint32_t phase = 0;
   int begun = kb;  // block of the set that this warp's sum starts at
@@ -469,6 +496,7 @@ __global__ void __launch_bounds__(kQgWarps* kWarp, T* NB <= 2 ? 2 : 1)
             if (p.w2) row_sums((j + T / 2) % T, i2, ulo, uhi);
             if (mine(i2)) {
               const int m = row0 + row_of(i2);
+              odd |= !isfinite(lo + hi) || (p.w2 && !isfinite(ulo + uhi));
               finish(p, m, set * cols + j * kQgTile + r, lo, ulo);
               finish(p, m, set * cols + j * kQgTile + r + 8, hi, uhi);
             }
@@ -517,7 +545,21 @@ __global__ void __launch_bounds__(kQgWarps* kWarp, T* NB <= 2 ? 2 : 1)
       v += d[0];
       if (p.w2) u += d[cols];
     }
+    odd |= !isfinite(v) || !isfinite(u);
     finish(p, row0 + m, (set0 + s) * cols + col, v, u);
+  }
+  // (rare: infinities that may have to be NaN)
+  if (!__syncthreads_or(odd)) return;
+#pragma unroll 1
+  for (int i = threadIdx.x; i < sets * rows << cl; i += blockDim.x) {
+    const int col = i & (cols - 1), sm = i >> cl, s = sm / rows, m = row0 + sm - s * rows;
+    const int n = (set0 + s) * cols + col;
+    const size_t at = (size_t)m * p.ldo + n;
+    if (n >= p.w.N || !isinf(load_out(p.out, at, p.a.type))) continue;
+    bool nan = false;
+#pragma unroll 1
+    for (int u = 0; u < (p.w2 ? 2 : 1) && !nan; ++u) nan = undefined_sum(p, u ? p.w2 : p.w.w, m, n);
+    if (nan) store_out(p.out, at, p.a.type, __uint_as_float(0x7fc00000u));
   }
 }
 

@@ -126,3 +126,75 @@ def test_a_large_channel_of_weights_zero_takes_no_bits(ctx, torch_cuda, M, large
         limit += 0.5 * 2.0 ** -23 * 4
     assert np.linalg.norm(c - exact) <= limit * np.linalg.norm(exact)
     w.close()
+
+
+def infinite_rows(torch, rng, K, dt):
+    """Rows with infinities at random: two to six in one group of k, one in
+    each of two groups, everywhere."""
+    x = rng.standard_normal((8, K))
+    for r in range(6):
+        at = rng.choice(32, size=2 + r % 5, replace=False) + 32 * (r % (K // 32))
+        x[r, at] = np.where(rng.random(len(at)) < 0.5, np.inf, -np.inf)
+    x[6, [3, K - 1]] = np.inf, -np.inf
+    x[7] = np.where(rng.random(K) < 0.5, np.inf, -np.inf)
+    return torch.from_numpy(x.astype(np.float32)).cuda().to(dt)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("M", [8, 24])
+@pytest.mark.parametrize("zeros,g,accumulate", [(False, 32, False), (True, 64, True), (True, 128, False)])
+def test_several_infinities_of_a_row(ctx, torch_cuda, M, dtype, zeros, g, accumulate):
+    """Infinities of opposite sign add up to NaN, of one sign to that infinity,
+    and one that meets a weight of 0 is NaN: as the definition has it, of few
+    rows and of many."""
+    torch = torch_cuda
+    from mojostream_b200.runtime import Q4GroupWeight
+    dt = getattr(torch, dtype)
+    rng = np.random.default_rng(M + g)
+    K, N = 384, 140
+    q, s, z = make_weight(rng, K, N, g, zeros)
+    s[:, 5::7] *= -1
+    if not zeros:
+        q[:, 20:60] = rng.choice([0x9a, 0xbc, 0xdf], size=(K, 40))  # one sign, no zeros
+    w = Q4GroupWeight(ctx, q, s, K, N, g, zeros=z)
+    x = torch.cat([infinite_rows(torch, rng, K, dt) for _ in range(M // 8)])
+    c = torch.ones((M, N), dtype=dt, device="cuda")
+    w.gemm(x, c, accumulate=accumulate)
+    with np.errstate(invalid="ignore"):
+        want = x.double().cpu().numpy() @ dense(q, s, z, g)
+    got = c.double().cpu().numpy()
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    fine = ~np.isnan(want)
+    assert np.isinf(want[fine]).all() and np.array_equal(got[fine], want[fine])
+    assert zeros or np.isinf(want).any()
+    w.close()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("M", [8, 24])
+@pytest.mark.parametrize("same", [False, True])
+def test_several_infinities_of_a_gated_row(ctx, torch_cuda, M, dtype, same):
+    torch = torch_cuda
+    from mojostream_b200.runtime import Q4GroupWeight
+    dt = getattr(torch, dtype)
+    rng = np.random.default_rng(M)
+    K, N, g = 256, 66, 64
+    mats = [make_weight(rng, K, N, g, False) for _ in range(2)]
+    for q, _, _ in mats:
+        q[:, 8:] = rng.choice([0x9a, 0xbc, 0xdf], size=(K, N // 2 - 8))
+    if same:
+        mats[1] = mats[0]
+    gate = Q4GroupWeight(ctx, *mats[0][:2], K, N, g)
+    up = gate if same else Q4GroupWeight(ctx, *mats[1][:2], K, N, g)
+    x = torch.cat([infinite_rows(torch, rng, K, dt) for _ in range(M // 8)])
+    x[0] = x[0].abs()
+    h = torch.empty((M, N), dtype=dt, device="cuda")
+    gate.gated(up, x, h)
+    a = x.double().cpu().numpy()
+    with np.errstate(invalid="ignore", over="ignore"):
+        v, u = (a @ dense(*m, g) for m in mats)
+        want = v / (1 + np.exp(-v)) * u  # (NaN for a gate of -infinity)
+    got = h.double().cpu().numpy()
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    fine = ~np.isnan(want)
+    assert fine[0, 16:].all() and np.array_equal(got[fine], want[fine])
