@@ -9,6 +9,7 @@
 
 #include "../../include/mojostream_cuda.h"
 #include "ms_internal.h"
+#include "ms_overlap.h"
 #include "ms_q4g.h"
 #include "ms_rules.h"
 
@@ -281,9 +282,7 @@ extern "C" ms_status ms_logit_rules_apply(ms_ctx* c, const void* logits, int64_t
   if (((uintptr_t)logits % es) || ((uintptr_t)out % es))
     OPS_FAIL(c, MS_ERR_ALIGN, "%s: logits must be aligned to their elements", what);
   // out either is logits or shares no byte with it
-  const uintptr_t a0 = (uintptr_t)logits, a1 = a0 + ((size_t)(M - 1) * ld + V) * es;
-  const uintptr_t b0 = (uintptr_t)out, b1 = b0 + ((size_t)(M - 1) * ldo + V) * es;
-  if (a0 != b0 && a0 < b1 && b0 < a1)
+  if (logits != out && rows_share((uintptr_t)logits, ld * es, V * es, (uintptr_t)out, ldo * es, V * es, M))
     OPS_FAIL(c, MS_ERR_INVALID_ARG, "%s: out overlaps logits without being it", what);
   const ms_logit_rules& q = *rules;
   if (!q.hist != !q.hist_off || !q.bias_id != !q.bias_off || !q.bias_id != !q.bias_val)
