@@ -164,7 +164,8 @@ MS_API ms_status ms_q4g_weight_destroy(ms_ctx *ctx, ms_q4g_weight *w);
 MS_API size_t ms_q4g_weight_bytes(const ms_q4g_weight *w);
 /* C[M,N] = A[M,K] . w (accumulate = 0) or C += A . w (accumulate = 1).
  * A and C: device memory of one type (dtype), rows lda >= K and ldc >= N
- * elements apart, aligned to their elements; they must not share memory.
+ * elements apart, aligned to their elements.  They must not share memory
+ * (MS_ERR_INVALID_ARG); column blocks of one buffer do not.
  * M <= 4194304.  Sums are fp32, rounded once to dtype.
  *   Few rows (up to 8 of fp32 and bfloat16, 16 of half): a value is held to
  * 2^-45 (fp32) or 2^-30 of the largest of its group in its row, at least

@@ -118,6 +118,8 @@ ms_status check_rows_args(ms_ctx* c, const char* what, const ms_q4g_weight* w, c
     OPS_FAIL(c, MS_ERR_ALIGN, "%s: A and the result must be aligned to their elements", what);
   if (!on_device(a, dev) || !on_device(out, dev))
     OPS_FAIL(c, MS_ERR_INVALID_ARG, "%s: A and the result must be memory of device %d", what, dev);
+  if (rows_share((uintptr_t)a, lda * es, w->v.K * es, (uintptr_t)out, ldo * es, w->v.N * es, M))
+    OPS_FAIL(c, MS_ERR_INVALID_ARG, "%s: A and the result share memory", what);
   return MS_OK;
 }
 

@@ -198,3 +198,29 @@ def test_several_infinities_of_a_gated_row(ctx, torch_cuda, M, dtype, same):
     assert np.array_equal(np.isnan(got), np.isnan(want))
     fine = ~np.isnan(want)
     assert fine[0, 16:].all() and np.array_equal(got[fine], want[fine])
+
+
+@pytest.mark.parametrize("M", [1, 4, 30])
+def test_operands_that_share_memory(ctx, torch_cuda, M):
+    """Products of A and C that share memory are refused and write nothing;
+    column blocks of one buffer share none."""
+    torch = torch_cuda
+    from mojostream_b200 import MsError
+    from mojostream_b200.runtime import Q4GroupWeight
+    rng = np.random.default_rng(M)
+    K, N, g = 128, 64, 64
+    q, s, z = make_weight(rng, K, N, g, True)
+    w = Q4GroupWeight(ctx, q, s, K, N, g, zeros=z)
+    buf = torch.from_numpy(rng.standard_normal((M + 1, K + N)).astype(np.float32)).cuda()
+    before = buf.clone()
+    for c in (buf[:M, :N], buf[:M, K - 1:K - 1 + N], buf[1:, 5:5 + N] if M > 1 else buf[:M, 7:7 + N]):
+        with pytest.raises(MsError, match="share memory"):
+            w.gemm(buf[:M, :K], c)
+        with pytest.raises(MsError, match="share memory"):
+            w.gated(w, buf[:M, :K], c)
+    assert torch.equal(buf, before)
+    want = w.gemm(before[:M, :K], torch.empty((M, N), device="cuda"))
+    w.gemm(buf[:M, :K], buf[:M, K:])
+    assert torch.equal(buf[:M, K:], want) and torch.equal(buf[:, :K], before[:, :K])
+    assert torch.equal(buf[M], before[M])
+    w.close()
