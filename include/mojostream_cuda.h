@@ -474,7 +474,8 @@ typedef struct {
 } ms_logit_rules;
 /* out[r] = rules(logits[r]); rows ld and ldo elements apart, of one type
  * (dtype).  out may be logits itself (then ld == ldo), else no row of the one
- * may overlap a row of the other (MS_ERR_INVALID_ARG).  M <= 65535.  Asynchronous; no workspace. */
+ * may overlap a row of the other (MS_ERR_INVALID_ARG).  M <= 65535; V, n_hist
+ * and n_bias <= 2^31 - 65537.  Asynchronous; no workspace. */
 MS_API ms_status ms_logit_rules_apply(ms_ctx *ctx, const void *logits, int64_t ld, void *out,
                                int64_t ldo, int dtype, int M, int V,
                                const ms_logit_rules *rules, void *stream);

@@ -291,6 +291,9 @@ extern "C" ms_status ms_logit_rules_apply(ms_ctx* c, const void* logits, int64_t
     OPS_FAIL(c, MS_ERR_INVALID_ARG, "%s: a list and its offsets go together", what);
   if (q.n_hist < 0 || q.n_bias < 0 || (!q.hist && q.n_hist) || (!q.bias_id && q.n_bias))
     OPS_FAIL(c, MS_ERR_INVALID_ARG, "%s: list lengths %d, %d", what, q.n_hist, q.n_bias);
+  // (a list is walked in steps of up to 4096 entries, by int)
+  if (q.n_hist > INT_MAX - 65536 || q.n_bias > INT_MAX - 65536)
+    OPS_FAIL(c, MS_ERR_SHAPE, "%s: list lengths %d, %d", what, q.n_hist, q.n_bias);
   if ((q.repetition || q.presence || q.frequency) && !q.hist)
     OPS_FAIL(c, MS_ERR_INVALID_ARG, "%s: penalties without a history", what);
   if (q.mask) {

@@ -44,3 +44,19 @@ def test_column_blocks_of_one_buffer(ctx, torch_cuda, M, V, dtype):
     assert torch.equal(torch.nan_to_num(buf[:, :V]), torch.nan_to_num(before))
     with pytest.raises(MsError, match="overlaps"):
         ctx.logit_rules(buf[:, :V], rules, out=buf[:, V - 1:2 * V - 1])
+
+
+@pytest.mark.parametrize("length", ["n_hist", "n_bias"])
+def test_lists_longer_than_their_walk_are_refused(ctx, torch_cuda, length):
+    """Indices of such a list would pass 2^31 behind its end: refused before
+    any launch, so nothing of the (short) list is read."""
+    torch = torch_cuda
+    from mojostream_b200 import MsError
+    rng = np.random.default_rng(1)
+    rules = on_gpu(torch, make(rng, 2, 100, 5, 5, 0))
+    lg = torch.zeros((2, 100), device="cuda")
+    for n in (2 ** 31 - 1, 2 ** 31 - 65536):
+        setattr(rules.desc, length, n)
+        with pytest.raises(MsError, match="MS_ERR_SHAPE.*list lengths"):
+            ctx.logit_rules(lg, rules)
+    assert not lg.any()
