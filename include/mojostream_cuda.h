@@ -176,7 +176,9 @@ MS_API size_t ms_q4g_weight_bytes(const ms_q4g_weight *w);
  *   The call may use the context's workspace: for each value of A (k rounded
  * up to 128) at most 8 (fp32) or 6 bytes with few rows; 2 (bfloat16), 4 (half)
  * or 6 (fp32) bytes with more, rounded up to whole tiles of 32 to 192 rows.
- * It grows on the first call of a size, which must not happen inside a stream
+ * It grows on the first call of a size, to twice what it was if that is more
+ * than the call needs and there is room for it; smaller ones that it replaced
+ * stay until ms_destroy.  A call that grows it must not be inside a stream
  * capture (MS_ERR_STATE), and calls on different streams must not overlap in
  * time, captured and replayed ones included. */
 MS_API ms_status ms_q4g_gemm(ms_ctx *ctx, const ms_q4g_weight *w, void *C, int64_t ldc,

@@ -34,6 +34,7 @@
 #include "ms_pages.h"
 #include "ms_plan.h"
 #include "ms_q4g.h"
+#include "ms_ws.h"
 
 using namespace ms;
 
@@ -424,12 +425,17 @@ ms_status ms_workspace_(ms_ctx* c, cudaStream_t s, size_t bytes, void** out) {
       return fail(c, MS_ERR_STATE,
                   "the workspace (%zu bytes) would have to grow to %zu inside a stream capture: "
                   "make one call of this size before it", c->ws_bytes, bytes);
-    const size_t want = std::max(std::max(bytes, 2 * c->ws_bytes), (size_t)1 << 20);
-    void* p = nullptr;
-    MS_TRY(dev_alloc(c, &p, want));
+    size_t got = 0;
+    void* p = ws_grow(bytes, c->ws_bytes, [](size_t n) {
+      void* q = nullptr;
+      if (cudaMalloc(&q, n) == cudaSuccess) return q;
+      cudaGetLastError();
+      return (void*)nullptr;
+    }, &got);
+    if (!p) return fail(c, MS_ERR_OOM, "no %zu bytes for the workspace", bytes);
     if (c->ws) c->ws_old.push_back(c->ws);
     c->ws = p;
-    c->ws_bytes = want;
+    c->ws_bytes = got;
   }
   *out = c->ws;
   return MS_OK;
