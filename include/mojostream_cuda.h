@@ -173,14 +173,17 @@ MS_API size_t ms_q4g_weight_bytes(const ms_q4g_weight *w);
  * passes the range of fp32 before its scale is applied (magnitudes near 2^117
  * and up) overflows to infinity or NaN; an infinity or NaN in a row of A makes
  * that row's results infinite or NaN as the formula does, and no other row's.
- *   The call may use the context's workspace: for each value of A (k rounded
+ *   The call may use a workspace of the context: for each value of A (k rounded
  * up to 128) at most 8 (fp32) or 6 bytes with few rows; 2 (bfloat16), 4 (half)
  * or 6 (fp32) bytes with more, rounded up to whole tiles of 32 to 192 rows.
- * It grows on the first call of a size, to twice what it was if that is more
- * than the call needs and there is room for it; smaller ones that it replaced
- * stay until ms_destroy.  A call that grows it must not be inside a stream
- * capture (MS_ERR_STATE), and calls on different streams must not overlap in
- * time, captured and replayed ones included. */
+ * Each stream that calls has one of its own (the last 16 of them: one more
+ * waits for the device), so calls on different streams may overlap in time.  It
+ * grows on the first call of a size, which waits for the stream, to twice what
+ * it was if that is more than the call needs and there is room for it.  A graph
+ * that the call is captured into has one too, until the graph and all made
+ * from it are gone, so graphs may run beside each other and beside other calls
+ * (but not two made from the same capture); MS_ERR_STATE if it is more than any
+ * call outside captures has asked for. */
 MS_API ms_status ms_q4g_gemm(ms_ctx *ctx, const ms_q4g_weight *w, void *C, int64_t ldc,
                       const void *A, int64_t lda, int dtype, int M, int accumulate,
                       void *stream);

@@ -22,7 +22,9 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <memory>
 #include <mutex>
+#include <new>
 #include <set>
 #include <string>
 #include <utility>
@@ -37,6 +39,44 @@
 #include "ms_ws.h"
 
 using namespace ms;
+
+// ------------------------------------------------------------ workspaces --
+
+namespace {
+struct WsDevice {  // of the current device; `s`: the stream of the call
+  cudaStream_t s;
+  static void* alloc(size_t n) {
+    void* p = nullptr;
+    if (cudaMalloc(&p, n) == cudaSuccess) return p;
+    cudaGetLastError();
+    return nullptr;
+  }
+  static void free(void* p) { cudaFree(p); }
+  void wait(unsigned long long) { cudaStreamSynchronize(s); }
+  static bool wait_all() {
+    if (cudaDeviceSynchronize() == cudaSuccess) return true;
+    cudaGetLastError();
+    return false;
+  }
+};
+struct RelaxedCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+struct WsGraphEnd {
+  std::shared_ptr<WsPool> pool;
+  unsigned long long graph;
+};
+void CUDART_CB ws_graph_end(void* p) {
+  auto* e = static_cast<WsGraphEnd*>(p);
+  try {
+    e->pool->release(e->graph);
+  } catch (...) {  // (host memory: the workspace stays the graph's until ms_destroy)
+  }
+  delete e;
+}
+}  // namespace
 
 // --------------------------------------------------------------- objects --
 
@@ -65,11 +105,8 @@ struct ms_ctx {
   // ms_sample: chunk partials and per-row arrival tickets (grown on demand)
   float2* samp_part = nullptr;
   size_t samp_part_n = 0;
-  // operators beside the token loop: one workspace, and the smaller ones that
-  // it replaced (captured graphs may hold them)
-  void* ws = nullptr;
-  size_t ws_bytes = 0;
-  std::vector<void*> ws_old;
+  // operators beside the token loop; captured graphs keep it beyond the context
+  std::shared_ptr<WsPool> ws = std::make_shared<WsPool>();
   double load_secs = 0.0;  // last ms_model_load: reads + host-to-device copies
   uint64_t load_bytes = 0;
   int* samp_cnt = nullptr;
@@ -397,8 +434,8 @@ extern "C" ms_status ms_destroy(ms_ctx* c) {
   cudaFree(c->rowf);
   cudaFree(c->samp_part);
   cudaFree(c->samp_cnt);
-  cudaFree(c->ws);
-  for (void* p : c->ws_old) cudaFree(p);
+  WsDevice ws_dev{nullptr};
+  c->ws->free_all(ws_dev);
   if (c->comm) nccl_api().comm_destroy(c->comm);
   if (c->ev[0]) cudaEventDestroy(c->ev[0]);
   if (c->ev[1]) cudaEventDestroy(c->ev[1]);
@@ -417,28 +454,51 @@ int ms_device_(const ms_ctx* c) { return c->device; }
 int ms_sm_count_(const ms_ctx* c) { return c->sm_count; }
 int* ms_err_word_(ms_ctx* c) { return c->d_err; }
 
-ms_status ms_workspace_(ms_ctx* c, cudaStream_t s, size_t bytes, void** out) {
-  if (bytes > c->ws_bytes) {
-    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    MS_CUDA(c, cudaStreamIsCapturing(s, &cap));
-    if (cap != cudaStreamCaptureStatusNone)
+static ms_status take_workspace(ms_ctx* c, cudaStream_t s, size_t bytes, void** out) {
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  unsigned long long graph = 0, stream = 0;
+  cudaGraph_t g = nullptr;
+  MS_CUDA(c, cudaStreamGetCaptureInfo(s, &cap, &graph, &g, nullptr, nullptr));
+  WsDevice dev{s};
+  if (cap == cudaStreamCaptureStatusNone) {
+    // (a handle may come again for another stream, an id does not)
+    MS_CUDA(c, cudaStreamGetId(s, &stream));
+    *out = c->ws->for_stream(stream, bytes, dev);
+  } else {
+    stream = (unsigned long long)(uintptr_t)s;  // (its id may not be asked for in a capture)
+    bool refused = false, first = false;
+    {
+      const RelaxedCapture relaxed;  // allocating memory is no operation of the capture
+      *out = c->ws->for_graph(graph, stream, bytes, dev, &refused, &first);
+    }
+    if (refused)
       return fail(c, MS_ERR_STATE,
-                  "the workspace (%zu bytes) would have to grow to %zu inside a stream capture: "
-                  "make one call of this size before it", c->ws_bytes, bytes);
-    size_t got = 0;
-    void* p = ws_grow(bytes, c->ws_bytes, [](size_t n) {
-      void* q = nullptr;
-      if (cudaMalloc(&q, n) == cudaSuccess) return q;
-      cudaGetLastError();
-      return (void*)nullptr;
-    }, &got);
-    if (!p) return fail(c, MS_ERR_OOM, "no %zu bytes for the workspace", bytes);
-    if (c->ws) c->ws_old.push_back(c->ws);
-    c->ws = p;
-    c->ws_bytes = got;
+                  "a workspace of %zu bytes inside a stream capture, where the largest so far is "
+                  "%zu: make one call of this size before it", bytes, c->ws->largest());
+    if (*out && first) {  // it comes back when the graph and all made from it are gone
+      cudaUserObject_t obj = nullptr;
+      auto* end = new (std::nothrow) WsGraphEnd{c->ws, graph};
+      cudaError_t e = end ? cudaUserObjectCreate(&obj, end, ws_graph_end, 1, cudaUserObjectNoDestructorSync)
+                          : cudaErrorMemoryAllocation;
+      if (e != cudaSuccess) {
+        c->ws->release(graph);
+        delete end;
+      } else if ((e = cudaGraphRetainUserObject(g, obj, 1, cudaGraphUserObjectMove)) != cudaSuccess) {
+        cudaUserObjectRelease(obj, 1);  // (its end returns the workspace)
+      }
+      MS_CUDA(c, e);
+    }
   }
-  *out = c->ws;
+  if (!*out) return fail(c, MS_ERR_OOM, "no %zu bytes for the workspace", bytes);
   return MS_OK;
+}
+
+ms_status ms_workspace_(ms_ctx* c, cudaStream_t s, size_t bytes, void** out) {
+  try {
+    return take_workspace(c, s, bytes, out);
+  } catch (const std::exception&) {
+    return fail(c, MS_ERR_OOM, "host memory for the workspace's bookkeeping");
+  }
 }
 
 void ms_set_load_stats_(ms_ctx* c, double seconds, uint64_t bytes) {

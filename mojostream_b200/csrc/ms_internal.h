@@ -1,5 +1,6 @@
 // Internal interface between the C-ABI core (ms_api.cu), the file loader
-// (ms_loader.cu) and the operators beside the token loop (ms_ops.cu).  Nothing here is exported from the library.
+// (ms_loader.cu) and the operators beside the token loop (ms_ops.cu).  Nothing
+// here is exported from the library.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -19,8 +20,7 @@ void ms_set_load_stats_(ms_ctx* c, double seconds, uint64_t bytes);
 int ms_sm_count_(const ms_ctx* c);
 // Device word of the error bits that bounded waits leave for ms_sync.
 int* ms_err_word_(ms_ctx* c);
-// At least `bytes` of the operators' device workspace, shared by all calls of
-// the context.  It grows by a new allocation; the old one lives until
-// ms_destroy, since captured graphs may hold it.  MS_ERR_STATE when it would
-// have to grow while `s` is being captured.
+// At least `bytes` of device workspace for one call on `s`: the stream's own, or
+// that of the graph which the stream is being captured into (ms_ws.h).
+// MS_ERR_STATE in a capture that asks for more than any call before it.
 ms_status ms_workspace_(ms_ctx* c, cudaStream_t s, size_t bytes, void** out);

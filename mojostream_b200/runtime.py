@@ -263,7 +263,9 @@ class Q4GroupWeight:
 
     def gemm(self, A, C, accumulate=False):
         """C = A . w, or C += A . w (ms_q4g_gemm): A [M][K] and C [M][N] of one
-        type (float32, bfloat16, float16), rows of any stride."""
+        type (float32, bfloat16, float16), rows of any stride, that share no
+        memory.  On torch's current stream; calls on several streams and
+        captured graphs keep workspaces of their own and may overlap."""
         ctx = self.ctx
         lda = _check_2d(A, "A", ctx.device, self.K)
         ldc = _check_2d(C, "C", ctx.device, self.N, A.shape[0])
@@ -276,7 +278,8 @@ class Q4GroupWeight:
 
     def gated(self, up, A, H, act="silu"):
         """H = act(A . self) * (A . up) in one kernel (ms_q4g_gated): the first
-        half of a gated feed-forward block; act "silu" or "gelu_tanh"."""
+        half of a gated feed-forward block; act "silu" or "gelu_tanh".  Streams
+        and graphs as gemm."""
         ctx = self.ctx
         lda = _check_2d(A, "A", ctx.device, self.K)
         ldh = _check_2d(H, "H", ctx.device, self.N, A.shape[0])
