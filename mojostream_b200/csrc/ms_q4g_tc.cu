@@ -42,6 +42,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <mutex>
+
 #include "ms_common.cuh"
 #include "ms_kernels.h"
 #include "ms_q4g.h"
@@ -873,7 +875,9 @@ cudaError_t prepare_q4g_tc() {
   if (e == cudaSuccess) e = prepare_tc_g<64>();
   if (e == cudaSuccess) e = prepare_tc_g<128>();
   if (e == cudaSuccess) e = prepare_tc_g<192>();
-  if (e == cudaSuccess && !g_clusters[1][1]) count_clusters();  // (every GPU of a node is alike)
+  // once (every GPU of a node is alike), and a context of another thread waits for it
+  static std::once_flag counted;
+  if (e == cudaSuccess) std::call_once(counted, count_clusters);
   return e;
 }
 
