@@ -168,8 +168,10 @@ MS_API size_t ms_q4g_weight_bytes(const ms_q4g_weight *w);
  * (MS_ERR_INVALID_ARG); column blocks of one buffer do not.
  * M <= 4194304.  Sums are fp32, rounded once to dtype.
  *   Few rows (up to 8 of fp32 and bfloat16, 16 of half): a value is held to
- * 2^-45 (fp32) or 2^-30 of the largest of its group in its row, at least
- * 2^-120.  More rows: values are used exactly as given.  A group whose sum
+ * 2^-45 (fp32) or 2^-30 of the largest of its group in its row, or to 2^-127
+ * (fp32) or 2^-120 where that is more.  More rows: values are used exactly as
+ * given, but fp32 to multiples of 2^-133, cut off (values from 2^-110 up are
+ * such multiples).  A group whose sum
  * passes the range of fp32 before its scale is applied (magnitudes near 2^117
  * and up) overflows to infinity or NaN; an infinity or NaN in a row of A makes
  * that row's results infinite or NaN as the formula does, and no other row's.

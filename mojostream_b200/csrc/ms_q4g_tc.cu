@@ -7,7 +7,8 @@
 // (the numbers up to 2^-125 are evenly spaced), so one fused multiply-add gives
 // (q - z) / 128 without a shift; the sums are multiplied by 128 at the end.
 // An activation is cut into bfloat16 limbs that add up to it exactly (fp32:
-// 8 + 8 + 8 bits, fp16: 8 + 3, bfloat16: itself), so every product of a
+// 8 + 8 + 8 bits, fp16: 8 + 3, bfloat16: itself; bits of fp32 below bfloat16's
+// least, 2^-133, are lost, which reaches values under 2^-110), so every product of a
 // tcgen05.mma is exact and its fp32 accumulator in tensor memory holds the sum
 // of one group of k over all limbs; when the group ends its scale is applied
 // and it is added to fp32 sums in registers.

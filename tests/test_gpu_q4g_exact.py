@@ -109,3 +109,25 @@ def test_a_small_value_beside_a_large_one(ctx, torch_cuda, dtype, M, g, zeros):
             tol = 2.0 ** -HELD[dtype] * largest[:, None] + 2.0 ** -BITS[dtype] * np.abs(want)
             assert (np.abs(got - want) <= tol).all(), gap
         h.close()
+
+
+@pytest.mark.parametrize("M", [1, 3, 8, 9, 24, 80, 200])
+def test_tiny_fp32_values(ctx, torch_cuda, M):
+    """Of few rows to half a step of 2^-126 where that is more than 2^-45 of the
+    largest; of many cut off to multiples of 2^-133, exact from 2^-110 up."""
+    torch = torch_cuda
+    rng = np.random.default_rng(M)
+    K, N = 128, 34
+    w = rng.choice([-1, 1], size=(K, N))
+    h = weight(ctx, w, 64, True, rng)
+    for e in (-100, -110, -112, -118, -124):
+        x, at = np.zeros((M, K)), rng.integers(0, K, M)
+        x[np.arange(M), at] = mantissas(rng, M, "float32") * 2.0 ** e
+        c = h.gemm(tensor(torch, x, "float32"), torch.empty((M, N), device="cuda")).double().cpu().numpy()
+        want = x[np.arange(M), at][:, None] * w[at]
+        err = np.abs(c - want)
+        if M <= 8:
+            assert (err <= np.maximum(2.0 ** -127, 2.0 ** -45 * np.abs(want))).all(), e
+        else:
+            assert (err < 2.0 ** -133).all() and (e < -110 or not err.any()), e
+    h.close()
