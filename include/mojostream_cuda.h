@@ -195,7 +195,11 @@ enum { MS_ACT_SILU = 0, MS_ACT_GELU_TANH = 1 };
 /* H[M,N] = act(A . gate) * (A . up), the first half of a gated feed-forward
  * block, in one kernel: neither product is written.  gate and up have the
  * same K, N, group and scale type, and both or neither have zero points
- * (MS_ERR_SHAPE otherwise).  The rest as ms_q4g_gemm. */
+ * (MS_ERR_SHAPE otherwise).  The activation is evaluated in fp32, for 16-bit
+ * results with approximate exponentials and reciprocals: a relative error of up
+ * to 2^-15 before the rounding to dtype, 2^-18 where the exponent is 8 or less
+ * in magnitude, so a result may be the next one where the exact value lies
+ * that near the middle of two.  The rest as ms_q4g_gemm. */
 MS_API ms_status ms_q4g_gated(ms_ctx *ctx, const ms_q4g_weight *gate, const ms_q4g_weight *up,
                        int act, void *H, int64_t ldh, const void *A, int64_t lda, int dtype,
                        int M, void *stream);

@@ -77,8 +77,9 @@ __device__ __forceinline__ float act_arg(float g, int act) {
   return act == 0 ? g : 2.f * 0.7978845608028654f * (g + 0.044715f * g * g * g);
 }
 __device__ __forceinline__ float act_wide(float g, int act) { return g / (1.f + expf(-act_arg(g, act))); }
-// For results of 16 bits: the approximate exponential (of a rounded argument x:
-// |x| 2^-24 relative, 2^-17 before the result vanishes) and reciprocal (2^-23).
+// For results of 16 bits: the approximate exponential (2^-22; of an argument x
+// with up to four roundings, |x| 2^-24 relative each: 2^-15 before the result
+// vanishes) and reciprocal (2^-23).  A 16-bit result has steps of 2^-8 or 2^-11.
 __device__ __forceinline__ float act_narrow(float g, int act) {
   float e, r;
   asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * act_arg(g, act)));

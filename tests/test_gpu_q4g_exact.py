@@ -131,3 +131,32 @@ def test_tiny_fp32_values(ctx, torch_cuda, M):
         else:
             assert (err < 2.0 ** -133).all() and (e < -110 or not err.any()), e
     h.close()
+
+
+@pytest.mark.parametrize("dtype", list(BITS))
+@pytest.mark.parametrize("M", [4, 64, 512])
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+def test_activations(ctx, torch_cuda, dtype, M, act):
+    """Rows with one value v, gate and up weights of 1: results act(v) v for v
+    over the range of the exponential.  Relative errors: the exponent x takes up
+    to four roundings (|x| 2^-24 each, as |x| 2^-24 of e^x), exponential,
+    sum and quotient 2^-21 together, the product one; then half a step."""
+    torch = torch_cuda
+    rng = np.random.default_rng(M)
+    K, N = 64, 2
+    dt = getattr(torch, dtype)
+    top = 80.0 if act == "silu" else 9.0
+    for low in (1e-3, 0.1, 1.0, top / 2):
+        v = rng.choice([-1.0, 1.0], M) * np.exp(rng.uniform(np.log(low), np.log(top), M))
+        a = torch.zeros((M, K), device="cuda", dtype=dt)
+        a[torch.arange(M), torch.from_numpy(rng.integers(0, K, M)).cuda()] = torch.from_numpy(v).cuda().to(dt)
+        v = a.sum(1).double().cpu().numpy()
+        w = weight(ctx, np.ones((K, N), np.int64), 64, False, rng)
+        got = w.gated(w, a, torch.empty((M, N), dtype=dt, device="cuda"), act=act).double().cpu().numpy()
+        x = v if act == "silu" else 2 * np.sqrt(2 / np.pi) * (v + 0.044715 * v ** 3)
+        want = v / (1 + np.exp(-x)) * v
+        rel = 4 * np.abs(x) * 2.0 ** -24 + 2.0 ** -21
+        assert rel.max() <= 2.0 ** -15 and (rel[np.abs(x) <= 8] <= 2.0 ** -18).all()
+        tol = np.abs(want) * (rel + 2.0 ** -BITS[dtype]) + torch.finfo(dt).smallest_normal * 2.0 ** -BITS[dtype]
+        assert (np.abs(got - want[:, None]) <= tol[:, None]).all(), low
+        w.close()
