@@ -470,11 +470,16 @@ __global__ void __launch_bounds__(kQgWarps* kWarp, T* NB <= 2 ? 2 : 1)
         }
       }
     }
-    // Every lane's loads from the stage have arrived before it is refilled: the
-    // last of them is in this sum, and a sum is never this NaN (a barrier alone
-    // does not wait for loads in flight)
-    const unsigned read = __ballot_sync(
-        0xffffffffu, __float_as_uint(acc[T - 1][NB - 1][1]) != 0x7fedcba9u);
+    // Every lane's loads from the stage have arrived before it is refilled: every
+    // tile's and every column block's are in this sum, and a sum is never this
+    // NaN (neither a barrier nor a later load's arrival says that an earlier
+    // load in flight has arrived)
+    float all = acc[T - 1][NB - 1][1];
+#pragma unroll
+    for (int j = 0; j < T - 1; ++j) all += acc[j][NB - 1][1];
+#pragma unroll
+    for (int b = 0; b < NB - 1; ++b) all += acc[T - 1][b][1];
+    const unsigned read = __ballot_sync(0xffffffffu, __float_as_uint(all) != 0x7fedcba9u);
     if (lane == 0 && read && i + p.stages < n) {
       issue_w(slot);
       if (!own_a) issue_a(slot, i_kb);

@@ -160,3 +160,29 @@ def test_many_streams_share_a_few_workspaces(torch_cuda):
             y.zero_()
     w.close()
     c2.close()
+
+
+@pytest.mark.parametrize("M,K,N,dtype", [(1, 2560, 20480, "bfloat16"), (1, 5120, 4096, "float32"),
+                                         (4, 10240, 2560, "bfloat16"), (3, 5120, 4096, "float32")])
+def test_few_rows_beside_many(ctx, torch_cuda, M, K, N, dtype):
+    """Decode calls while another stream's products of 64 rows keep the SMs'
+    shared memory busy, so that loads from a ring's stages take longest when
+    the stages are refilled."""
+    torch = torch_cuda
+    w, a, alone, out = jobs(torch, ctx, M, K, N, dtype, 2)
+    w2, a2, alone2, out2 = jobs(torch, ctx, 64, 5120, 2048, "bfloat16", 1)
+    one, other = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(30):
+        for y in out + out2:
+            y.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(other):
+            for _ in range(10):
+                w2.gemm(a2[0], out2[0])
+        with torch.cuda.stream(one):
+            for _ in range(8):
+                for x, y in zip(a, out):
+                    w.gemm(x, y)
+        torch.cuda.synchronize()
+        for y, want in zip(out + out2, alone + alone2):
+            assert torch.equal(y, want)
