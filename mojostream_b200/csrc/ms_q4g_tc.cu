@@ -31,15 +31,20 @@
 // cluster's CTAs share the k of one; their sums are added in k order through
 // distributed shared memory.
 // The loops are kept short: with unrolled limbs and the next stage's waits among
-// the MMAs 2048 rows (K 2560, N 10240, bfloat16) took 137 us, and take 99 us
-// (1085 TFLOP/s; 4096 x 5120 x 13824 537 us, 1080 TFLOP/s), with the
-// activation's exact division unrolled 519 gated rows took 114 us, and take 97.
+// the MMAs 2048 rows (K 2560, N 10240, bfloat16) took 137 us, and take 98 us
+// (1095 TFLOP/s; inputs that are not in L2 113 us; 4096 x 5120 x 13824 537 us,
+// 1080 TFLOP/s), with the activation's exact division unrolled 519 gated rows took
+// 114 us, and take 99.
 //
-// What bounds it: many rows, the MMAs (at their measured rate 65 of the 99 us)
+// What bounds it: many rows, the MMAs (at their measured rate 65 of the 98 us)
 // and the hand-over between the roles; a quarter of the planes' bytes (58 KB a
 // block come from L2) would save 9 us, no writing of results as much.  Few rows:
-// the instructions that unpack (64 gated rows, K 5120, N 13824: 52 us; 42 us
-// without those that shifted and subtracted, a third of which is gone since).
+// a chain of 1.2 us per block of 128 k (an unpacking warp waits for its stage,
+// unpacks, stores to tensor memory, waits for the store, arrives and only then
+// takes the next block's words), the same in tiles of 32 and of 64 rows though
+// there a warp unpacks twice as much (64 gated rows, K 5120, N 13824, 40 blocks
+// a CTA: 48 us, issue slots taken for 61 % of the active cycles, the tensor pipe
+// for 21 %).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
