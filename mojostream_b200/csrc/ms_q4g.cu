@@ -579,16 +579,17 @@ StreamPlan plan_stream(const Q4gParams& p, int sm_count) {
   const int row_blocks = (p.a.M + per - 1) / per;
   o.NB = (per * digits + 7) / 8;
   // four tiles to a set share a block's loads and loop (one row, K 2560, N
-  // 20480: 7.6 us, with two 8.6 us) where the GPU still gets a set per SM;
-  // fewer columns fill it better with two (N 2560: 4.5 us, with four 4.6 us).
+  // 20480 bfloat16: 7.0 us, with two 8.8 us) where the GPU still gets a set per
+  // SM; fewer columns fill it better with two (three rows, N 2560: 6.5 us, with
+  // four 7.1 us).
   // From five rows (three of fp32) on four tiles' sums do not fit the registers.
   const int quads = q4g_quads(p.w.N) * (p.w2 ? 2 : 1);
   o.T = o.NB <= 2 && quads >= sm_count ? 4 : 2;
   o.sets = quads * kQgQuad / o.T;
   // rows x blocks that 16 warps convert in two rounds (one or two rows: three,
-  // more fp32 rows: one); more come converted, a launch more (one row, K 10240, N
-  // 5120 bfloat16: 14.4 us, and 17.3 us; four rows, K 2560: 8.1 and 7.3 us; fp32,
-  // four rows, K 1280: 6.0 and 5.5 us)
+  // more fp32 rows: one); more come converted, a launch more (one row, K 2560, N
+  // 20480 bfloat16: 7.0 us, and 7.8 us; four rows, N 2560: 7.5 and 5.5 us; fp32,
+  // four rows, K 1280, N 2560: 6.0 and 5.5 us)
   const size_t rec = (size_t)qg_record_bytes(per * digits, p.w.group);
   const size_t a_all = p.w.nkb * rec;
   o.a_smem = row_blocks == 1 && per * p.w.nkb <= (per <= 2 ? 6 : digits == 6 ? 2 : 4) * kQgWarps && a_all <= 64 * 1024 ? a_all : 0;
