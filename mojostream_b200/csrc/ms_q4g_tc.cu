@@ -10,8 +10,8 @@
 // 8 + 8 + 8 bits, fp16: 8 + 3, bfloat16: itself; bits of fp32 below bfloat16's
 // least, 2^-133, are lost, which reaches values under 2^-110), so every product of a
 // tcgen05.mma is exact and its fp32 accumulator in tensor memory holds the sum
-// of one group of k over all limbs; when the group ends its scale is applied
-// and it is added to fp32 sums in registers.
+// of one group of k over all limbs (fp32 rows: of at most 64 k); when it ends the
+// group's scale is applied and it is added to fp32 sums in registers.
 //
 // CTA: tiles of 128 weight columns on the MMA's M side (gated: 64 of the gate,
 // 64 of the up weight, in turns of 16) x NT rows on its N side x a share of the
@@ -208,7 +208,8 @@ __device__ __forceinline__ void reg_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-// NT: rows of the tile; G: 32-k steps per group.
+// NT: rows of the tile; G: 32-k steps that an accumulator sums (a group's, or of
+// fp32 rows two of a group of four).
 template <int NT, int G>
 __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
     q4g_tc_kernel(const Q4gParams p, const TcShape c) {
@@ -443,7 +444,7 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
     const uint32_t ta = tmem_a + ((uint32_t)(quad * kWarp + j0 * 16) << 16) + (HS == 2 ? half * 32 : 0);
     // the tiles among a stage's eight
     const int piece = p.w2 ? quad + 4 * j0 : 2 * quad + j0, piece_step = (p.w2 ? 4 : 1) * bb;
-    constexpr int ng = 4 / G;
+    const int ng = kQgBlockK / p.w.group;
     Ring rs, rw;
     if (HS == 1) rs.next(c.nS, half);
     int n = 0, left = blocks;
@@ -459,7 +460,7 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
         if (p.w.zeros)
 #pragma unroll
           for (int hh = 0; hh < 2; ++hh)
-            z[j][hh] = lds16(pc + j * piece_step + kQgNibbles + ng * 32 + ((2 * half + hh) / G * 8 + r) * 2);
+            z[j][hh] = lds16(pc + j * piece_step + kQgNibbles + ng * 32 + ((2 * half + hh) * ng / 4 * 8 + r) * 2);
       }
       return true;
     };
@@ -527,12 +528,13 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
       const bool exists = un.second || piece < 4;
       const uint8_t* scales = (piece < 4 ? un.w0 : un.w1) + (piece & 3) * bb + kQgNibbles +
                               ((lane & 7) * 2 + ((lane >> 3) & 1)) * 2;
-      uint2 sn = make_uint2(0, 0);  // the block's ng scales
+      const int second = G == 2 && p.w.group == 128 ? 0 : 16;  // (two sums of a group: its scale again)
+      uint2 sn = make_uint2(0, 0);  // the scales of the block's ng sums
       auto fetch = [&]() {
         const unsigned short* q = reinterpret_cast<const unsigned short*>(scales);
         if (exists) {
           sn.x = __ldg(q);
-          if (ng > 1) sn.x |= (uint32_t)__ldg(q + 16) << 16;
+          if (ng > 1) sn.x |= (uint32_t)__ldg(q + second) << 16;
           if (ng > 2) sn.y = __ldg(q + 32) | (uint32_t)__ldg(q + 48) << 16;
         }
         scales += run;
@@ -801,7 +803,10 @@ cudaError_t launch_tc_g(const Q4gParams& p, const TcPlan& o, cudaStream_t s) {
   switch (p.w.group) {
     case 32: return launch_tc_t<NT, 1>(p, o, s);
     case 64: return launch_tc_t<NT, 2>(p, o, s);
-    default: return launch_tc_t<NT, 4>(p, o, s);
+    // fp32: two sums of 64 k to a group, so that the low limbs of its second half
+    // are not cut off against the first half's sum (the error of 20 rows, K 256:
+    // 0.7e-7, with one sum 2.6e-7)
+    default: return o.c.limbs == 3 ? launch_tc_t<NT, 2>(p, o, s) : launch_tc_t<NT, 4>(p, o, s);
   }
 }
 

@@ -224,3 +224,23 @@ def test_operands_that_share_memory(ctx, torch_cuda, M):
     assert torch.equal(buf[:M, K:], want) and torch.equal(buf[:, :K], before[:, :K])
     assert torch.equal(buf[M], before[M])
     w.close()
+
+
+@pytest.mark.parametrize("M", [9, 20, 50, 300])
+def test_fp32_sums_of_long_groups_keep_their_last_bits(ctx, torch_cuda, M):
+    """A group of 128 as two sums of 64, each with the bound of the test before:
+    one sum would cut the second half's small limbs off against the first half
+    (eight more cuts of half a unit at 0.7 of the group's size)."""
+    torch = torch_cuda
+    from mojostream_b200.runtime import Q4GroupWeight
+    rng = np.random.default_rng(M)
+    K, N, g = 256, 512, 128
+    q, s, z = make_weight(rng, K, N, g, True)
+    w = Q4GroupWeight(ctx, q, s, K, N, g, zeros=z)
+    a = torch.from_numpy(rng.standard_normal((M, K)).astype(np.float32)).cuda()
+    c = w.gemm(a, torch.empty((M, N), device="cuda")).double().cpu().numpy()
+    exact = a.double().cpu().numpy() @ dense(q, s, z, g)
+    cuts = 0.5 * 2.0 ** -23 * sum(((j + 1) / 4) ** 0.5 for j in range(4))
+    limit = cuts + 2.0 ** -24 / 3 ** 0.5 * ((K // 64 + 1) / 2) ** 0.5
+    assert np.linalg.norm(c - exact) <= limit * np.linalg.norm(exact)
+    w.close()
