@@ -208,9 +208,9 @@ __device__ __forceinline__ void reg_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-// NT: rows of the tile; G: 32-k steps that an accumulator sums (a group's, or of
-// fp32 rows two of a group of four).
-template <int NT, int G>
+// NT: rows of the tile; G: 32-k steps that an accumulator sums: a group's, or
+// (`parts`, fp32 rows) two of a group of four.
+template <int NT, int G, bool parts = false>
 __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
     q4g_tc_kernel(const Q4gParams p, const TcShape c) {
   using S_ = Tile<NT>;
@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
     const uint32_t ta = tmem_a + ((uint32_t)(quad * kWarp + j0 * 16) << 16) + (HS == 2 ? half * 32 : 0);
     // the tiles among a stage's eight
     const int piece = p.w2 ? quad + 4 * j0 : 2 * quad + j0, piece_step = (p.w2 ? 4 : 1) * bb;
-    const int ng = kQgBlockK / p.w.group;
+    constexpr int ng = parts ? 1 : 4 / G;  // groups of a block
     Ring rs, rw;
     if (HS == 1) rs.next(c.nS, half);
     int n = 0, left = blocks;
@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(Tile<NT>::kThreads, Tile<NT>::kCtas)
       const bool exists = un.second || piece < 4;
       const uint8_t* scales = (piece < 4 ? un.w0 : un.w1) + (piece & 3) * bb + kQgNibbles +
                               ((lane & 7) * 2 + ((lane >> 3) & 1)) * 2;
-      const int second = G == 2 && p.w.group == 128 ? 0 : 16;  // (two sums of a group: its scale again)
+      constexpr int second = parts ? 0 : 16;  // (two sums of a group: its scale again)
       uint2 sn = make_uint2(0, 0);  // the scales of the block's ng sums
       auto fetch = [&]() {
         const unsigned short* q = reinterpret_cast<const unsigned short*>(scales);
@@ -775,7 +775,7 @@ TcPlan plan_tc(const Q4gParams& p, int sm_count) {
   return o;
 }
 
-template <int NT, int G>
+template <int NT, int G, bool parts = false>
 cudaError_t launch_tc_t(const Q4gParams& p, const TcPlan& o, cudaStream_t s) {
   if (!o.smem) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg = {};
@@ -795,7 +795,7 @@ cudaError_t launch_tc_t(const Q4gParams& p, const TcPlan& o, cudaStream_t s) {
     attr[1].val.clusterDim.z = 1;
     cfg.numAttrs = 2;
   }
-  return cudaLaunchKernelEx(&cfg, q4g_tc_kernel<NT, G>, p, o.c);
+  return cudaLaunchKernelEx(&cfg, q4g_tc_kernel<NT, G, parts>, p, o.c);
 }
 
 template <int NT>
@@ -803,10 +803,13 @@ cudaError_t launch_tc_g(const Q4gParams& p, const TcPlan& o, cudaStream_t s) {
   switch (p.w.group) {
     case 32: return launch_tc_t<NT, 1>(p, o, s);
     case 64: return launch_tc_t<NT, 2>(p, o, s);
-    // fp32: two sums of 64 k to a group, so that the low limbs of its second half
-    // are not cut off against the first half's sum (the error of 20 rows, K 256:
-    // 0.7e-7, with one sum 2.6e-7)
-    default: return o.c.limbs == 3 ? launch_tc_t<NT, 2>(p, o, s) : launch_tc_t<NT, 4>(p, o, s);
+    default:
+      // fp32: two sums of 64 k to a group, so that the low limbs of its second half
+      // are not cut off against the first half's sum (the error of 20 rows, K 256:
+      // 0.7e-7, with one sum 2.6e-7); never in tiles of 192 rows, which have one limb
+      if constexpr (NT <= 128)
+        if (o.c.limbs == 3) return launch_tc_t<NT, 2, true>(p, o, s);
+      return launch_tc_t<NT, 4>(p, o, s);
   }
 }
 
@@ -838,16 +841,18 @@ void count_clusters() {
     }
 }
 
-template <int NT, int G>
+template <int NT, int G, bool parts = false>
 cudaError_t prepare_tc_t() {
-  return cudaFuncSetAttribute(q4g_tc_kernel<NT, G>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              (int)kTqSmemMax);
+  return cudaFuncSetAttribute(q4g_tc_kernel<NT, G, parts>,
+                              cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTqSmemMax);
 }
 template <int NT>
 cudaError_t prepare_tc_g() {
   cudaError_t e = prepare_tc_t<NT, 1>();
   if (e == cudaSuccess) e = prepare_tc_t<NT, 2>();
   if (e == cudaSuccess) e = prepare_tc_t<NT, 4>();
+  if constexpr (NT <= 128)
+    if (e == cudaSuccess) e = prepare_tc_t<NT, 2, true>();
   return e;
 }
 
